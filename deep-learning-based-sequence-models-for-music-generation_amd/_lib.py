@@ -107,6 +107,15 @@ SIGNATURES = {
     "msq_mamba_ssd_step": (_i, [_p, _i64, _p, _p, _i64, _p, _i64, _i, _p, _p, _p, _i64, _i64, _i64, _p]),
     "msq_filtered_logit_step": (_i, [_p, _i64, _p, _p, _i, _i64, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _p]),
     "msq_mamba_conv_bwd":(_i, [_p, _p, _i64, _p, _i64, _i, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _p]),
+    "msq_kv8_blocks": (_i64, [_i64, _i64]),
+    "msq_kv8_write": (_i, [_i, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _p, _i64,
+                           _p]),
+    "msq_kv8_read": (_i, [_i, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p]),
+    "msq_relattn_decode_kv8_workspace": (_sz, [_i64, _i64, _i64, _i64]),
+    "msq_relattn_decode_kv8": (_i, [_i, _p, _i64, _p, _i64, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _i64,
+                                    _i64, _p, _i64, _f, _p, _sz, _p]),
+    "msq_token_logprobs": (_i, [_p, _p, _p, _p, _p, _p, _i, _i64, _p, _i64, _i64, _i64, _p]),
+    "msq_token_logprobs_bwd": (_i, [_p, _i64, _p, _p, _p, _p, _p, _p, _i64, _p, _i, _i64, _p, _i64, _i64, _p]),
     "msq_relattn_bwd_workspace": (_sz, [_i, _i64, _i64, _i64]),
     "msq_relattn_bwd": (_i, [_i, _p, _i64, _p, _p, _i64, _p, _p, _p, _i64, _p, _i64, _i64, _i64, _i64, _i64, _f, _i64,
                              _p, _p]),
@@ -163,6 +172,14 @@ def ptr(t):
 
 def stream():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+def on_current(dev):
+    """raises unless dev is the GPU whose current stream a launch would go to"""
+    if dev.type != "cuda":
+        raise RuntimeError("the MI355X kernels run on the GPU only (no CPU fallback)")
+    if dev.index != torch.cuda.current_device():
+        raise ValueError(f"tensors on {dev} while cuda:{torch.cuda.current_device()} is the current device")
 
 
 def dt(t):

@@ -3,7 +3,7 @@ models/transformer/model_transformer.py:41-90) over the libmidiseq C ABI."""
 import torch
 
 from . import _lib as L
-from ._lib import ptr, call, stream, dt
+from ._lib import ptr, call, stream, dt, on_current
 from .ops import workspace
 
 N_META = 6  # metadata prefix (generate_matrix, model_transformer.py:14)
@@ -49,3 +49,115 @@ def relattn_bwd(dout, out, lse, qkv, R, B, S, H, hs, scale, dqkv=None, dR=None, 
          ptr(ws), ready, stream())
     _ws_served[slot] = (ws.data_ptr(), key)
     return dqkv, dR
+
+
+# ---- the decode cache in 8 bits (msq_kv8_*, msq_relattn_decode_kv8)
+
+KV8_BLOCK = 64  # slots that share a scale
+
+
+def kv8_cache(B, H, S_ring, hs, device="cuda", block=KV8_BLOCK, layers=()):
+    """An empty 8-bit ring (kc, ks, vc, vs): e4m3 codes [*layers, B, H, S_ring,
+    hs] and fp32 scales [*layers, B, H, ceil(S_ring / block)] of the keys and of
+    the values."""
+    nblk = L.lib().msq_kv8_blocks(S_ring, block)
+    if nblk < 0:
+        raise ValueError(f"a ring of {S_ring} slots in blocks of {block} (16, 32, 64 or 128)")
+    if hs <= 0 or hs > 128 or hs % 8:
+        raise ValueError(f"head size {hs}: the 8-bit cache needs 8 | hs <= 128")
+    codes = [torch.zeros(*layers, B, H, S_ring, hs, device=device, dtype=torch.uint8).view(torch.float8_e4m3fn)
+             for _ in range(2)]
+    scales = [torch.ones(*layers, B, H, nblk, device=device, dtype=torch.float32) for _ in range(2)]
+    return codes[0], scales[0], codes[1], scales[1]
+
+
+def _kv8_args(kc, ks, vc, vs, pos, n_meta, block, *others):
+    """the checked cache: (pointers, (B, H, hs, S_ring, n_meta, block, pos, pos_stride))"""
+    if kc.dtype != torch.float8_e4m3fn or vc.dtype != kc.dtype or kc.dim() != 4 or kc.shape != vc.shape:
+        raise ValueError(f"the cache is two float8_e4m3fn [B, H, S_ring, hs] tensors, got {kc.dtype} "
+                         f"{tuple(kc.shape)} and {vc.dtype} {tuple(vc.shape)}")
+    B, H, S_ring, hs = kc.shape
+    if not 0 <= n_meta < S_ring or block not in (16, 32, 64, 128):
+        raise ValueError(f"a ring of {S_ring} slots, {n_meta} of them metadata, in blocks of {block}")
+    want = (B, H, -(-S_ring // block))
+    if ks.dtype != torch.float32 or vs.dtype != torch.float32 or ks.shape != want or vs.shape != want:
+        raise ValueError(f"the scales are two float32 {list(want)} tensors, got {ks.dtype} {tuple(ks.shape)} and "
+                         f"{vs.dtype} {tuple(vs.shape)}")
+    if not (kc.is_contiguous() and vc.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
+        raise ValueError("the cache and its scales have to be contiguous")
+    n = pos.numel()
+    if pos.dtype != torch.int64 or pos.dim() > 1 or (n != 1 and n != B) or not pos.is_contiguous():
+        raise ValueError(f"pos is an int64 tensor of 1 or {B} positions, got {pos.dtype} {tuple(pos.shape)}")
+    dev = kc.device
+    for t in (vc, ks, vs, pos) + others:
+        if t.device != dev:
+            raise ValueError(f"tensors on {dev} and {t.device}")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in others):
+        raise ValueError("the 8-bit cache has no gradient: call it under torch.no_grad()")
+    return (ptr(kc), ptr(ks), ptr(vc), ptr(vs)), (B, H, hs, S_ring, n_meta, block, ptr(pos), 0 if n == 1 else 1)
+
+
+def kv8_write(kc, ks, vc, vs, k, v, pos, *, n_meta=N_META, block=KV8_BLOCK):
+    """Writes new keys and values k, v [B, T, H, hs] (fp32 / bf16; heads hs
+    apart, any other strides, the same for both: e.g. views of a packed
+    projection) at positions pos .. pos + T - 1 of the ring, in place
+    (msq_kv8_write). pos: int64 [B], or [1] for all rows; -n_meta for a prompt
+    whose first n_meta rows are metadata; below that a row is left alone."""
+    if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.stride() != v.stride():
+        raise ValueError(f"k and v are [B, T, H, hs] alike, got {k.dtype} {tuple(k.shape)} {k.stride()} and "
+                         f"{v.dtype} {tuple(v.shape)} {v.stride()}")
+    cache, (B, H, hs, *rest) = _kv8_args(kc, ks, vc, vs, pos, n_meta, block, k, v)
+    T = k.shape[1]
+    if k.shape != (B, T, H, hs) or k.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError(f"{k.dtype} {tuple(k.shape)} rows for a cache of {B} x {H} heads of {hs}")
+    if (hs > 1 and k.stride(3) != 1) or (H > 1 and k.stride(2) != hs):
+        raise ValueError(f"a token's heads have to lie {hs} apart, got strides {k.stride()}")
+    on_current(kc.device)
+    if T == 0:
+        return
+    call("msq_kv8_write", dt(k), *cache, ptr(k), ptr(v), k.stride(0), k.stride(1), B, T, H, hs, *rest, stream())
+
+
+def kv8_read(kc, ks, vc, vs, pos, *, first=0, rows=None, dtype=torch.bfloat16, n_meta=N_META, block=KV8_BLOCK):
+    """Keys and values of the windows whose newest position is pos, oldest row
+    first: rows first .. first + rows - 1 (default: all that a window can hold)
+    as [B, H, rows, hs] in dtype, zeros past a row's window (msq_kv8_read)."""
+    cache, (B, H, hs, S_ring, *rest) = _kv8_args(kc, ks, vc, vs, pos, n_meta, block)
+    rows = S_ring - first if rows is None else rows
+    if first < 0 or rows < 0 or first + rows > S_ring or dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError(f"rows {first} .. {first + rows} of a ring of {S_ring} in {dtype}")
+    on_current(kc.device)
+    k = torch.empty(B, H, rows, hs, device=kc.device, dtype=dtype)
+    v = torch.empty_like(k)
+    if rows:
+        call("msq_kv8_read", dt(k), ptr(k), ptr(v), *cache, B, H, hs, S_ring, *rest, first, rows, stream())
+    return k, v
+
+
+def relattn_decode_kv8(q, kc, ks, vc, vs, R, pos, scale, *, out=None, n_meta=N_META, block=KV8_BLOCK):
+    """One decode position of the relative attention over the 8-bit cache, whose
+    newest position is pos (msq_relattn_decode_kv8): q [B, H, hs] (heads hs
+    apart), R [H, S_max, hs] contiguous, both fp32 or bf16. Returns out [B, H,
+    hs] in that type; rows that are not in use (pos < -n_meta) get zeros."""
+    if q.dim() != 3 or q.dtype not in (torch.float32, torch.bfloat16) or R.dtype != q.dtype:
+        raise ValueError(f"q [B, H, hs] and R in fp32 or bf16, got {q.dtype} {tuple(q.shape)} and {R.dtype}")
+    if out is None:
+        out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+    cache, (B, H, hs, S_ring, *rest) = _kv8_args(kc, ks, vc, vs, pos, n_meta, block, q, R, out)
+    if q.shape != (B, H, hs) or R.dim() != 3 or R.shape[0] != H or R.shape[1] < S_ring or R.shape[2] != hs:
+        raise ValueError(f"q {tuple(q.shape)} and R {tuple(R.shape)} for a cache of {B} x {H} x {S_ring} x {hs}")
+    if out.shape != q.shape or out.dtype != q.dtype:
+        raise ValueError(f"out {out.dtype} {tuple(out.shape)} for q {q.dtype} {tuple(q.shape)}")
+    for t in (q, out):
+        if (hs > 1 and t.stride(2) != 1) or (H > 1 and t.stride(1) != hs):
+            raise ValueError(f"a row's heads have to lie {hs} apart, got strides {t.stride()}")
+    if not R.is_contiguous():
+        raise ValueError("R has to be contiguous")
+    on_current(kc.device)
+    n = L.lib().msq_relattn_decode_kv8_workspace(B, H, hs, S_ring)
+    # a scratch of its own for every call: captured graphs and streams never share one
+    ws = torch.empty(n, device=q.device, dtype=torch.uint8) if n else None
+    call("msq_relattn_decode_kv8", dt(q), ptr(out), out.stride(0) if B > 1 else H * hs, ptr(q),
+         q.stride(0) if B > 1 else H * hs, *cache, ptr(R), R.shape[1], B, H, hs, S_ring, *rest, float(scale), ptr(ws), n,
+         stream())
+    return out

@@ -29,6 +29,9 @@ Cached mode (``mode="cached"``):
   ``context_len`` tokens; filtered_logit's time-axis LSE runs over the
   window's cached logits rows. oracle/transformer.py CachedTransformer
   restates these semantics; tests/test_decode_cached_gpu.py pins the build to it.
+  ``kv="fp8"`` holds the ring's keys and values in 8 bits (e4m3 codes, a
+  power-of-two scale per 64 slots and head): half the bytes a step reads, at one
+  rounding of 2^-4 relative per key / value element.
 
 Sharded decode (``group=``): the global batch of world x B
 prompts is split by rows over the ranks of a process group, one model
@@ -49,7 +52,7 @@ import torch.distributed as dist
 from . import _lib as L
 from ._lib import ptr, call, stream, dt
 from .config import Grammar
-from .loss import grammar_table
+from .loss import filtered_logit, grammar_table, token_logprobs
 from .ops import workspace
 
 
@@ -97,7 +100,7 @@ class _Shard:
 
 @torch.no_grad()
 def generate(model, context_len, token_ids, meta_ids, num_tokens=1000, device="cuda", rng=None, uniforms=None,
-             grammar: Grammar = None, return_tensor=False, mode="exact", group=None):
+             grammar: Grammar = None, return_tensor=False, mode="exact", group=None, kv=None):
     """Returns a list of B token lists of length T0 + num_tokens (like the
     reference). ``rng`` defaults to the global ``random`` module (as in the
     reference); ``uniforms`` is an optional iterator of floats (one per row
@@ -105,7 +108,8 @@ def generate(model, context_len, token_ids, meta_ids, num_tokens=1000, device="c
     torch.Generator is used. ``group`` (a torch.distributed process group, or
     True for the default one): this call decodes this rank's B rows of a
     sharded batch of world x B rows (module docstring); ``rng``, ``uniforms``
-    (world x B per step) and torch's seed must then be the same on every rank."""
+    (world x B per step) and torch's seed must then be the same on every rank.
+    ``kv="fp8"``: the Transformer's cached decode with keys and values in 8 bits."""
     grammar = grammar or Grammar()
     rng = rng or _random
     eng = model.engine
@@ -129,6 +133,8 @@ def generate(model, context_len, token_ids, meta_ids, num_tokens=1000, device="c
     if mode not in ("exact", "cached"):
         raise ValueError(f"mode must be 'exact' or 'cached', not {mode!r}")
     cached = mode == "cached"
+    if kv is not None and not (cached and getattr(eng, "cache_slides", False)):
+        raise ValueError(f"kv={kv!r} goes with the Transformer's mode='cached'")
     slides = cached and getattr(eng, "cache_slides", False)  # Transformer: stays cached past the context
     cache = None
     ldz = (V + 3) // 4 * 4
@@ -167,7 +173,7 @@ def generate(model, context_len, token_ids, meta_ids, num_tokens=1000, device="c
         else:
             window = hist[:, cur - W:cur].contiguous()
             if cached and cache is None and (cur <= context_len or slides):  # prefill, states left in the cache
-                cache = eng.decode_cache(B, context_len) if slides else eng.decode_cache(B)
+                cache = eng.decode_cache(B, context_len, kv) if slides else eng.decode_cache(B)
                 logits = eng.forward(window, meta_ids, save=False, cache=cache)
                 col_lse = cache.lse
             else:
@@ -218,3 +224,19 @@ def generate(model, context_len, token_ids, meta_ids, num_tokens=1000, device="c
         last_host = tok_host.tolist()
     seq = hist[:, :T0 + num_tokens]
     return seq if return_tensor else seq.tolist()
+
+
+@torch.no_grad()
+def score(model, token_ids, meta_ids, top=0, grammar: Grammar = None, device="cuda"):
+    """How likely the model finds given rows, e.g. generated ones: for tokens 1 ..
+    T of token_ids [B, T + 1] (T <= block_len) under the reference's filtered
+    distribution softmax(Z), Z = filtered_logit(tokens 0 .. T-1, logits) (train.py:
+    133-138), the loss.TokenLogprobs [B, T]: log probability, entropy and the
+    ``top`` alternatives. The mean of -logprob is the training loss of the rows."""
+    dev = torch.device(device)
+    token_ids = token_ids.to(dev)
+    src, trg = token_ids[:, :-1].contiguous(), token_ids[:, 1:].contiguous()
+    if src.shape[1] == 0:
+        raise ValueError("score needs rows of two tokens or more")
+    logits = model.engine.forward(src, meta_ids.to(dev).contiguous(), save=False)
+    return token_logprobs(filtered_logit(src, logits, grammar), trg, top)

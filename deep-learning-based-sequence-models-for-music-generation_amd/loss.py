@@ -6,11 +6,18 @@
 * ``filtered_cross_entropy(src, logits, trg)`` fuses filtered_logit and the
   cross-entropy (mean over B*T, no ignore_index) into one pass and produces
   d(loss)/d(logits) in the same pass when gradients are needed.
-No [B,T,V] weight tensor is ever materialised."""
+No [B,T,V] weight tensor is ever materialised.
+
+* ``token_logprobs(logits, tokens, top)``: log probability of given tokens,
+  entropy and the top alternatives of rows of logits (csrc/logprobs.hip,
+  autograd supported)."""
+from typing import NamedTuple, Optional
+
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib as L
-from ._lib import ptr, call, stream, dt
+from ._lib import ptr, call, stream, dt, on_current
 from .config import Grammar
 from .ops import workspace
 
@@ -132,3 +139,79 @@ def _padded(t):
 def filtered_logit(input, output, grammar: Grammar = None):
     """train.py:133-138 drop-in: -log_softmax(output, dim=1) * weights[bucket(input)]."""
     return _FilteredLogit.apply(output, input, grammar)
+
+
+class TokenLogprobs(NamedTuple):
+    logprob: torch.Tensor                  # fp32 [...]
+    entropy: torch.Tensor                  # fp32 [...]
+    top_ids: Optional[torch.Tensor]        # int64 [..., top] (None: top = 0)
+    top_logprobs: Optional[torch.Tensor]   # fp32 [..., top]
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, tokens, top):
+        rows, V = x.shape
+        f32 = dict(device=x.device, dtype=torch.float32)
+        lp, ent = torch.empty(rows, **f32), torch.empty(rows, **f32)
+        need = ctx.needs_input_grad[0]
+        stats = torch.empty(rows, 2, **f32) if need else None
+        ids = torch.empty(rows, top, device=x.device, dtype=torch.int64) if top else None
+        top_lp = torch.empty(rows, top, **f32) if top else None
+        call("msq_token_logprobs", ptr(lp), ptr(ent), ptr(stats), ptr(ids), ptr(top_lp), ptr(x), dt(x), x.stride(0),
+             ptr(tokens), rows, V, top, stream())
+        if need:
+            ctx.save_for_backward(x, tokens, stats, ent, ids)
+            ctx.top = top
+            ctx.set_materialize_grads(False)
+            if top:
+                ctx.mark_non_differentiable(ids)
+        return lp, ent, ids, top_lp
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_lp, g_ent, _, g_top):
+        x, tokens, stats, ent, ids = ctx.saved_tensors
+        if g_lp is None and g_ent is None and g_top is None:
+            return None, None, None
+        rows, V = x.shape
+        # rows of the gradient as far apart as those of x where that only pads
+        # them: both then meet the same 16-byte boundaries
+        ld = x.stride(0) if V <= x.stride(0) < V + 64 else V
+        dx = torch.empty(rows, ld, device=x.device, dtype=x.dtype)[:, :V]
+        g = [None if t is None else t.to(torch.float32).contiguous() for t in (g_lp, g_ent, g_top)]
+        call("msq_token_logprobs_bwd", ptr(dx), ld, ptr(g[0]), ptr(g[1]), ptr(g[2]), ptr(stats), ptr(ent), ptr(ids),
+             ctx.top, ptr(x), dt(x), x.stride(0), ptr(tokens), rows, V, stream())
+        return dx, None, None
+
+
+def token_logprobs(logits, tokens, top=0):
+    """Of every row of logits [..., V] (fp32 / bf16; e.g. the model's logits or
+    filtered_logit's Z): the log probability of its token (int64 [...]; outside
+    [0, V), e.g. -100: 0 and no gradient), the entropy, and the ids and log
+    probabilities of the ``top`` <= 32 largest logits (equal ones by index).
+    logprob, entropy and top_logprobs are differentiable in logits. A row of
+    nothing but -inf gives log probability -inf, entropy 0 and no gradient; NaN
+    or +inf makes its row NaN."""
+    V = logits.shape[-1] if logits.dim() else 0
+    if logits.dtype not in (torch.float32, torch.bfloat16) or V == 0:
+        raise ValueError(f"logits [..., V] in fp32 or bf16, got {logits.dtype} {tuple(logits.shape)}")
+    if tokens.dtype != torch.int64 or tokens.shape != logits.shape[:-1]:
+        raise ValueError(f"int64 tokens {list(logits.shape[:-1])}, got {tokens.dtype} {tuple(tokens.shape)}")
+    if not 0 <= top <= min(32, V):
+        raise ValueError(f"{top} alternatives of {V} (at most 32)")
+    if tokens.device != logits.device:
+        raise ValueError(f"logits on {logits.device}, tokens on {tokens.device}")
+    on_current(logits.device)
+    shape = tuple(tokens.shape)
+    if tokens.numel() == 0:  # no rows: empty results, on the graph of logits
+        z = logits.sum(-1).float()
+        t = logits[..., :top].float()
+        return TokenLogprobs(z, z.clone(), torch.empty(t.shape, device=t.device, dtype=torch.int64) if top else None,
+                             t if top else None)
+    x = logits.reshape(-1, V)
+    if x.stride(1) != 1:
+        x = x.contiguous()
+    lp, ent, ids, top_lp = _TokenLogprobs.apply(x, tokens.reshape(-1).contiguous(), top)
+    return TokenLogprobs(lp.view(shape), ent.view(shape), ids.view(shape + (top,)) if top else None,
+                         top_lp.view(shape + (top,)) if top else None)

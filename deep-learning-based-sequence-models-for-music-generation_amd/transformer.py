@@ -23,7 +23,7 @@ import torch.nn as nn
 from . import _lib as L
 from . import ops
 from ._lib import ptr, call, stream, dt
-from .attention import relattn_fwd, relattn_bwd
+from .attention import kv8_cache, kv8_read, kv8_write, relattn_bwd, relattn_decode_kv8, relattn_fwd
 from .config import N_META, VOCAB_SIZE, METADATA_VOCAB_SIZE, BLOCK_LEN, DROPOUT
 
 # dropout sites of the counter-based keep masks (csrc/common.h; oracle/dropout.py):
@@ -214,19 +214,28 @@ class TransformerDecodeCache:
     hs], a ring: metadata in slots 0..5, sequence position p in slot
     6 + p % context), the window's logits rows (a ring [B, context, v_pad],
     empty rows -inf so they drop out of the time-axis LSE) and tokens, and the
-    one-position step buffers."""
+    one-position step buffers. kv="fp8": the keys / values as e4m3 codes with a
+    power-of-two scale per (64 slots, head) instead (attention.kv8_cache), half
+    the bytes of the bf16 ring."""
 
     slides = True  # keeps stepping once the window is full (the Mamba cache does not)
 
-    def __init__(self, cfg, B, context, device, act):
+    def __init__(self, cfg, B, context, device, act, kv=None):
         d, H, hs = cfg.n_embd, cfg.n_heads, cfg.head_size
+        if kv not in (None, "fp8"):
+            raise ValueError(f"kv must be None (the engine's type) or 'fp8', not {kv!r}")
         if context + N_META > cfg.s_max:
             raise ValueError(f"context {context} exceeds block_len {cfg.block_len}")
         f32 = torch.float32
         e = lambda *s, dt=act: torch.empty(*s, device=device, dtype=dt)  # noqa: E731
         self.B, self.ctx, self.S_ring = B, context, context + N_META
-        self.k = torch.zeros(cfg.n_layer, B, H, self.S_ring, hs, device=device, dtype=act)
-        self.v = torch.zeros_like(self.k)
+        self.act, self.kv8 = act, kv == "fp8"
+        if self.kv8:
+            self.k, self.k_scale, self.v, self.v_scale = kv8_cache(B, H, self.S_ring, hs, device, layers=(cfg.n_layer,))
+            self.prefill_pos = torch.full((1,), -N_META, device=device, dtype=torch.int64)
+        else:
+            self.k = torch.zeros(cfg.n_layer, B, H, self.S_ring, hs, device=device, dtype=act)
+            self.v = torch.zeros_like(self.k)
         self.ring = torch.full((B, context, cfg.v_pad), float("-inf"), device=device, dtype=act)
         self.tokens = torch.zeros(B, context, device=device, dtype=torch.int64)
         self.lse = e(B, cfg.vocab_size, dt=f32)
@@ -255,6 +264,24 @@ class TransformerDecodeCache:
         self.pos_dev = torch.zeros(1, device=device, dtype=torch.int64)
         self.row_buf = e(B, cfg.v_pad)
         self.graph, self.graph_gen, self.tok_buf = None, None, None
+
+    def layer8(self, l):
+        """layer l of an 8-bit cache: (codes, scales) of the keys and of the values"""
+        return self.k[l], self.k_scale[l], self.v[l], self.v_scale[l]
+
+    def window_kv(self, l, dtype=None):
+        """Layer l's keys and values of the window, oldest row first (metadata in
+        front): two [B, H, n, hs] in dtype (default: the engine's type), n = N_META +
+        min(length, ctx)."""
+        dtype = dtype or self.act
+        n = N_META + min(self.length, self.ctx)
+        if self.kv8:
+            last = torch.full((1,), self.length - 1, device=self.k.device, dtype=torch.int64)
+            return kv8_read(*self.layer8(l), last, rows=n, dtype=dtype)
+        slots = torch.arange(n, device=self.k.device)
+        if self.length > self.ctx:
+            slots[N_META:] = N_META + (slots[N_META:] - N_META + self.length) % self.ctx
+        return self.k[l][:, :, slots].to(dtype), self.v[l][:, :, slots].to(dtype)
 
     def stage_tok(self, tok):
         """the step graph's token buffer (int64 [B]) holding tok; a new buffer
@@ -430,6 +457,9 @@ class TransformerEngine:
             ops.gemm(A.a[k], W[f"{l}.wqkv"], out=A.qkv[k])
             if cache is not None:
                 kv = A.qkv[k].view(B, S, 3, H, hs)
+                if cache.kv8:
+                    kv8_write(*cache.layer8(l), kv[:, :, 1], kv[:, :, 2], cache.prefill_pos)
+            if cache is not None and not cache.kv8:
                 cache.k[l][:, :, :S].copy_(kv[:, :, 1].transpose(1, 2))
                 cache.v[l][:, :, :S].copy_(kv[:, :, 2].transpose(1, 2))
             adrop = pdrop = fdrop = None
@@ -476,8 +506,9 @@ class TransformerEngine:
             cache.pos_dev.fill_(T)
         return A.logits.view(B, T, cfg.v_pad)[:, :, :V]
 
-    def decode_cache(self, B, context=None):
-        return TransformerDecodeCache(self.cfg, B, context or self.cfg.block_len, self.device, self.act)
+    def decode_cache(self, B, context=None, kv=None):
+        """kv="fp8": keys and values in 8 bits (else in the engine's type)"""
+        return TransformerDecodeCache(self.cfg, B, context or self.cfg.block_len, self.device, self.act, kv)
 
     # decode steps after the first replay one captured HIP graph
     # (False: eager launches with host-side positions; tests / profiling)
@@ -537,6 +568,15 @@ class TransformerEngine:
             nxt = (P[f"{l + 1}.ln1_w"], P[f"{l + 1}.ln1_b"], cache.a) if l + 1 < L_ else (P["lnf_w"], P["lnf_b"], cache.f)
             ops.gemm_resid_ln(cache.h, W[f"{l}.w2"], x, P[f"{l}.b2"], cache.xm, *nxt)
 
+    def _attn8(self, l, cache):
+        """the decode attention of layer l over the 8-bit cache, the new token's keys
+        and values (at position cache.pos_dev) written first"""
+        B, H, hs = cache.B, self.cfg.n_heads, self.cfg.head_size
+        qkv = cache.qkv.view(B, 1, 3, H, hs)
+        kv8_write(*cache.layer8(l), qkv[:, :, 1], qkv[:, :, 2], cache.pos_dev)
+        relattn_decode_kv8(qkv[:, 0, 0], *cache.layer8(l), self.W[f"{l}.R"], cache.pos_dev, self.cfg.n_embd ** -0.5,
+                           out=cache.o.view(B, H, hs))
+
     def _step_dev(self, tok, cache):
         """step() with every position-dependent quantity read from cache.pos_dev"""
         cfg, P, W = self.cfg, self.P, self.W
@@ -546,6 +586,8 @@ class TransformerEngine:
         call("msq_embed_fwd", ptr(cache.x), ptr(P["tok_emb"]), ptr(P["meta_emb"]), ptr(tok), None, B, 1, 0, d, s)
 
         def attn(l):
+            if cache.kv8:
+                return self._attn8(l, cache)
             call("msq_relattn_decode_pos", dt(cache.qkv), ptr(cache.o), cache.o.stride(0), ptr(cache.qkv),
                  cache.qkv.stride(0), ptr(cache.k[l]), ptr(cache.v[l]), ptr(W[f"{l}.R"]), cfg.s_max, B, H, hs,
                  cache.S_ring, N_META, ptr(cache.pos_dev), float(scale), ptr(cache.attn_ws), cache.attn_ws.numel(), s)
@@ -573,10 +615,13 @@ class TransformerEngine:
         call("msq_embed_fwd", ptr(cache.x), ptr(P["tok_emb"]), ptr(P["meta_emb"]), ptr(tok), None, B, 1, 0, d, s)
 
         def attn(l):
+            if cache.kv8:
+                return self._attn8(l, cache)
             call("msq_relattn_decode", dt(cache.qkv), ptr(cache.o), cache.o.stride(0), ptr(cache.qkv),
                  cache.qkv.stride(0), ptr(cache.k[l]), ptr(cache.v[l]), ptr(W[f"{l}.R"]), cfg.s_max, B, H, hs,
                  cache.S_ring, N_META, n_tok, N_META + slot, first % ctx, float(scale), ptr(cache.attn_ws),
                  cache.attn_ws.numel(), s)
+        cache.pos_dev.fill_(pos)
         self._layers_step(cache.x, cache, attn)
         ops.gemm(cache.f, W["lm_w"], out=cache.row_buf, epilogue=L.EPI_BIAS, bias=P["lm_b"])
         if not cache.part_valid:  # first step: every block partial of the prefilled window
@@ -584,7 +629,6 @@ class TransformerEngine:
                  cfg.vocab_size, cache.RB, 0, cache.nblk, slot, -1, s)
             cache.ring_blk.fill_(-1)
             cache.part_valid = True
-        cache.pos_dev.fill_(pos)
         self._ring_step(tok, cache)
         cache.length = pos + 1
         cache.logits = cache.row_buf

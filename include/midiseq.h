@@ -488,6 +488,66 @@ int msq_relattn_decode_pos(int dtype, void* out, int64_t ldo, const void* qkv, i
                            int64_t n_meta, const int64_t* pos, float scale, void* ws, size_t ws_bytes,
                            void* stream);
 
+/* ---- the decode cache in 8 bits -------------------------------------------
+ * The cached decode's keys / values (what scripts/generate.py:26-31 recomputes
+ * per token) as e4m3 codes [B, H, S_ring, hs] with one fp32 power-of-two scale
+ * per (block of slots, head), [B, H, msq_kv8_blocks(S_ring, block)]. The ring is
+ * msq_relattn_decode's: metadata position s - n_meta (negative) in slot
+ * s < n_meta, the token at position p >= 0 in slot n_meta + p % (S_ring -
+ * n_meta); a row whose newest position is `last` holds S = n_meta + min(last +
+ * 1, ctx) keys, none where that is <= 0. block: 16, 32, 64 or 128 slots;
+ * 8 | hs <= 128; cache pointers 8-B aligned. pos: int64 on the device, one
+ * per row of the batch (pos_stride 1) or one for all (0); a row with pos <
+ * -n_meta is not in use: its cache is left alone and its attention is 0.
+ * Slots behind a row's last one are neither read nor written, whatever they hold. */
+int64_t msq_kv8_blocks(int64_t S_ring, int64_t block);
+/* T new rows of keys and values (dtype MSQ_F32 / MSQ_BF16; row t of batch row b
+ * at k + b * ld_b + t * ld_t, head h at + h * hs) become positions pos .. pos +
+ * T - 1; positions are written in order. A touched block's scale becomes the
+ * smallest 2^e, e >= -126, with |x| <= 448 * 2^e over its finite contents, new
+ * rows and rows that stay; rows that stay are coded again where the scale
+ * moved (exact but for codes that fall under 2^-6 of the new scale).
+ * Infinities saturate, NaN stays NaN.                                        */
+int msq_kv8_write(int dtype, void* kc, float* ks, void* vc, float* vs, const void* k, const void* v, int64_t ld_b,
+                  int64_t ld_t, int64_t B, int64_t T, int64_t H, int64_t hs, int64_t S_ring, int64_t n_meta,
+                  int64_t block, const int64_t* pos, int64_t pos_stride, void* stream);
+/* Rows first .. first + rows - 1 of every window, oldest first (metadata rows in
+ * front), in dtype into k, v [B, H, rows, hs]; zeros past a row's window. pos =
+ * the newest position written.                                               */
+int msq_kv8_read(int dtype, void* k, void* v, const void* kc, const float* ks, const void* vc, const float* vs,
+                 int64_t B, int64_t H, int64_t hs, int64_t S_ring, int64_t n_meta, int64_t block, const int64_t* pos,
+                 int64_t pos_stride, int64_t first, int64_t rows, void* stream);
+/* msq_relattn_decode_pos over that cache, after msq_kv8_write of the step's keys
+ * and values: out[b, h] = softmax_j((q.k_j + q.R[w(j)]) * scale) . v_j over the
+ * window of row b's newest position pos; q [B, ldq] and out [B, ldo] with head h
+ * at h * hs, R [H, S_max, hs], all in dtype; w(j) = key j's place in the window.
+ * ws of msq_relattn_decode_kv8_workspace(...) bytes, 16-B aligned (0: none).  */
+size_t msq_relattn_decode_kv8_workspace(int64_t B, int64_t H, int64_t hs, int64_t S_ring);
+int msq_relattn_decode_kv8(int dtype, void* out, int64_t ldo, const void* q, int64_t ldq, const void* kc,
+                           const float* ks, const void* vc, const float* vs, const void* R, int64_t S_max, int64_t B,
+                           int64_t H, int64_t hs, int64_t S_ring, int64_t n_meta, int64_t block, const int64_t* pos,
+                           int64_t pos_stride, float scale, void* ws, size_t ws_bytes, void* stream);
+
+/* ---- log probabilities of given tokens ------------------------------------
+ * For each of `rows` rows of V logits (row stride ld >= 0, any alignment): logprob
+ * = log softmax(x)[token], entropy of softmax(x), and (top > 0, <= 32) the ids
+ * and log probabilities [rows, top] of the largest logits, equal ones by index,
+ * NaN largest: the row terms of CrossEntropyLoss (train_parallel.py:156,179)
+ * and torch.topk (scripts/generate.py:66-74). A token outside [0, V) (padding)
+ * gets 0; a row of nothing but -inf gets logprob -inf and entropy 0. stats
+ * (fp32 [rows, 2]: row maximum, log of the scaled sum) is kept for the backward
+ * (NULL: not wanted).                                                        */
+int msq_token_logprobs(float* logprob, float* entropy, float* stats, int64_t* top_ids, float* top_logprobs,
+                       const void* logits, int dtype, int64_t ld, const int64_t* tokens, int64_t rows, int64_t V,
+                       int64_t top, void* stream);
+/* dlogits (dtype, row stride ldd; overwritten) = the gradient of sum(g_logprob *
+ * logprob) + sum(g_entropy * entropy) + sum(g_top * top_logprobs); each g_ fp32
+ * or NULL. stats, entropy and top_ids as the forward left them.               */
+int msq_token_logprobs_bwd(void* dlogits, int64_t ldd, const float* g_logprob, const float* g_entropy,
+                           const float* g_top, const float* stats, const float* entropy, const int64_t* top_ids,
+                           int64_t top, const void* logits, int dtype, int64_t ld, const int64_t* tokens, int64_t rows,
+                           int64_t V, void* stream);
+
 /* Note -> token encode of a batch of songs (replaces processing/processing.py
  * :129-152 encode + :111-126 adjust_note_time, the preprocessing step of
  * preprocess_midi_files :24-55). Song s = notes [song_off[s], song_off[s+1])
