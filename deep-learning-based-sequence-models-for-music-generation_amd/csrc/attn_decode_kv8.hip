@@ -5,17 +5,19 @@
 // over the S keys of the row's window, w(j) = the key's position in it (slot j
 // itself until the ring wraps). Rows whose window is empty get zeros.
 //
-// Split over the keys: one workgroup per (chunk of slots, h, b); a key is
-// spread over a 16-lane group, 8 values per lane, and every group keeps its own
-// running maximum and sum (one pass, no exchange inside the loop); the groups
-// and waves are joined at the end, the chunks by a second kernel.
+// Bound by the cache's bytes (2 hs per key and (b, h)); R comes from L2.
+// Split over the keys (flash decoding): one workgroup of 4 waves per (chunk of
+// slots, h, b). A key is spread over LPK lanes, VPL values each (16-byte loads of
+// 16 codes where the head size allows it), so a wave's load covers 64 / LPK
+// consecutive slots; every such key group keeps its own running maximum, sum and
+// output (one pass, no exchange inside the loop but the LPK-lane sum of a
+// score). Groups and waves are joined at the end, chunks by a second kernel.
 #include "kv8.h"
 
 namespace {
 
-constexpr int NT = 256, HS = KV8_MAX_HS, GROUPS = 16, UN = 4, STEP = GROUPS * UN;
-
-typedef float f32x8 __attribute__((ext_vector_type(8)));
+constexpr int NT = 256, HS = KV8_MAX_HS;
+constexpr float LOG2E = 1.44269504088896340736f;
 
 struct Args {
     const void* q;
@@ -26,113 +28,201 @@ struct Args {
     float *po, *pml;
     const int64_t* pos;
     int64_t pos_stride, ldq, ldo, S_max;
-    int H, hs, S_ring, n_meta, block, nblk, chunk, nsplit;
+    int B, H, hs, S_ring, n_meta, block_log2, nblk, chunk, nsplit, remap;
     float scale;
 };
 
-__device__ __forceinline__ f32x8 ld8(const bf16* p) {
-    const bf16x8 x = *(const bf16x8*)p;
-    return (f32x8){(float)x[0], (float)x[1], (float)x[2], (float)x[3], (float)x[4], (float)x[5], (float)x[6], (float)x[7]};
-}
-__device__ __forceinline__ f32x8 ld8(const float* p) {
-    const f32x4 a = *(const f32x4*)p, b = *(const f32x4*)(p + 4);
-    return (f32x8){a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-}
-__device__ __forceinline__ f32x8 ld8(const uint8_t* p) {
-    const uint2 x = *(const uint2*)p;
-    const f32x4 a = kv8_dec4(x.x), b = kv8_dec4(x.y);
-    return (f32x8){a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-}
 // 2^(x - m) with an empty maximum read as 0 (x is then -inf too)
 __device__ __forceinline__ float pexp(float x, float m) {
     return __builtin_amdgcn_exp2f(x - (m == -INFINITY ? 0.f : m));
 }
 
-template <typename T>
+// N values of a row as the lane holds them
+template <typename T, int N> struct Row;
+template <int N> struct Row<bf16, N> {
+    u32x4 v[N / 8];
+    __device__ __forceinline__ void load(const bf16* p) {
+#pragma unroll
+        for (int i = 0; i < N / 8; ++i) v[i] = ((const u32x4*)p)[i];
+    }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < N / 8; ++i) v[i] = (u32x4){0u, 0u, 0u, 0u};
+    }
+    __device__ __forceinline__ bf16x2 pair(int i) const {
+        const uint32_t x = v[i >> 2][i & 3];  // a value: __builtin_bit_cast of a vector's element reads element 0
+        return __builtin_bit_cast(bf16x2, x);
+    }
+    __device__ __forceinline__ float dot(const Row& o) const {
+        float a = 0.f;
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) a = __builtin_amdgcn_fdot2_f32_bf16(pair(i), o.pair(i), a, false);
+        return a;
+    }
+};
+template <int N> struct Row<float, N> {
+    f32x4 v[N / 4];
+    __device__ __forceinline__ void load(const float* p) {
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) v[i] = ((const f32x4*)p)[i];
+    }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) v[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    }
+    __device__ __forceinline__ float dot(const Row& o) const {
+        float a = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) a = fmaf(v[i >> 2][i & 3], o.v[i >> 2][i & 3], a);
+        return a;
+    }
+};
+template <int N> struct Codes {
+    uint32_t v[N / 4];
+    __device__ __forceinline__ void load(const uint8_t* p) {
+        if constexpr (N == 16) {
+            const u32x4 x = *(const u32x4*)p;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = x[i];
+        } else {
+            const uint2 x = *(const uint2*)p;
+            v[0] = x.x, v[1] = x.y;
+        }
+    }
+    // e4m3 is exact in bf16: two products per instruction
+    __device__ __forceinline__ float dot(const Row<bf16, N>& q) const {
+        float a = 0.f;
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) {
+            a = __builtin_amdgcn_fdot2_f32_bf16(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[i], 1.f, false),
+                                                q.pair(2 * i), a, false);
+            a = __builtin_amdgcn_fdot2_f32_bf16(__builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(v[i], 1.f, true),
+                                                q.pair(2 * i + 1), a, false);
+        }
+        return a;
+    }
+    __device__ __forceinline__ float dot(const Row<float, N>& q) const {
+        float a = 0.f;
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) {
+            const f32x4 c = kv8_dec4(v[i]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) a = fmaf(c[e], q.v[i][e], a);
+        }
+        return a;
+    }
+    __device__ __forceinline__ void add_to(float* o, float p) const {
+#pragma unroll
+        for (int i = 0; i < N / 4; ++i) {
+            const f32x4 c = kv8_dec4(v[i]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[4 * i + e] = fmaf(p, c[e], o[4 * i + e]);
+        }
+    }
+};
+
+template <typename T, int VPL, int LPK>
 __global__ __launch_bounds__(NT) void decode_kv8_kernel(Args a) {
+    constexpr int GW = 64 / LPK;                       // keys per load of a wave
+    constexpr int UN = VPL * sizeof(T) > 32 ? 2 : 4;   // loads of a wave in flight: 64 registers
+    constexpr int STEP = 4 * GW * UN;
     __shared__ float part[4][HS];
     __shared__ float wm[4], wl[4];
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    const int l16 = lane & 15, grp = w * 4 + (lane >> 4);
-    const int c = blockIdx.x, h = blockIdx.y, hs = a.hs, ctx = a.S_ring - a.n_meta;
-    const int64_t b = blockIdx.z, bh = b * a.H + h;
-    const int64_t last = a.pos[b * a.pos_stride];
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, grp = lane / LPK;
+    // the rows of the batch that read the same rows of R run side by side on one
+    // XCD ((h, chunk) pairs dealt round the 8 of them)
+    int h, c;
+    int64_t b;
+    if (a.remap) {
+        const int i = blockIdx.x >> 3, pair = i / a.B * 8 + (blockIdx.x & 7);
+        if (pair >= a.H * a.nsplit) return;
+        b = i % a.B;
+        h = pair / a.nsplit;
+        c = pair % a.nsplit;
+    } else {
+        b = blockIdx.x % a.B;
+        const int pair = blockIdx.x / a.B;
+        h = pair / a.nsplit;
+        c = pair % a.nsplit;
+    }
+    const int hs = a.hs, ctx = a.S_ring - a.n_meta;
+    const int64_t bh = b * a.H + h, last = a.pos[b * a.pos_stride];
     const int S = kv8_window(last, a.n_meta, ctx), first = kv8_first(last, ctx), s0 = c * a.chunk;
-    if (s0 >= S && a.nsplit > 1) return;  // chunk past the window (uniform)
-    const int d0 = 8 * l16;
+    const int n = min(S - s0, a.chunk);  // keys of this chunk
+    const int d0 = VPL * (lane % LPK);
     const bool dok = d0 < hs;
-    const uint8_t* kc = a.kc + bh * a.S_ring * hs + d0;
-    const uint8_t* vc = a.vc + bh * a.S_ring * hs + d0;
+    const uint8_t* kc = a.kc + (bh * a.S_ring + s0) * hs + d0;
+    const uint8_t* vc = a.vc + (bh * a.S_ring + s0) * hs + d0;
     const float *ks = a.ks + bh * a.nblk, *vs = a.vs + bh * a.nblk;
     const T* R = (const T*)a.R + (int64_t)h * a.S_max * hs + d0;
-    f32x8 q = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (dok) q = ld8((const T*)a.q + b * a.ldq + (int64_t)h * hs + d0);
-    const float sc = a.scale * 1.44269504088896340736f;  // scores in base 2
+    Row<T, VPL> q;
+    q.zero();
+    if (dok) q.load((const T*)a.q + b * a.ldq + (int64_t)h * hs + d0);
+    const float sc = a.scale * LOG2E;  // scores in base 2
 
-    float m = -INFINITY, l = 0.f, o[8];
+    float m = -INFINITY, l = 0.f, o[VPL];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] = 0.f;
-    const int s1 = min(S, s0 + a.chunk);
-    for (int t = s0; t < s1; t += STEP) {
-        float x[UN];
-        f32x8 v[UN];
+    for (int e = 0; e < VPL; ++e) o[e] = 0.f;
+    for (int t = w * GW * UN; t < n; t += STEP) {
+        Codes<VPL> k[UN], v[UN];
+        Row<T, VPL> r[UN];
+        float fk[UN], fv[UN];
 #pragma unroll
         for (int u = 0; u < UN; ++u) {
-            const int s = min(t + u * GROUPS + grp, s1 - 1);  // rows past the chunk: masked below
-            int j = s;
-            if (s >= a.n_meta) {
+            const int s = min(t + u * GW + grp, n - 1);  // rows past the chunk: masked below
+            int j = s0 + s;
+            fk[u] = ks[j >> a.block_log2];
+            fv[u] = vs[j >> a.block_log2];
+            if (j >= a.n_meta) {
                 j -= first;
                 j += j < a.n_meta ? ctx : 0;
             }
-            float acc = 0.f, rel = 0.f;
-            v[u] = q;
             if (dok) {
-                const f32x8 k = ld8(kc + (int64_t)s * hs), r = ld8(R + (int64_t)j * hs);
-                v[u] = ld8(vc + (int64_t)s * hs);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) acc = fmaf(k[e], q[e], acc), rel = fmaf(r[e], q[e], rel);
+                k[u].load(kc + (uint32_t)(s * hs));
+                r[u].load(R + (int64_t)j * hs);
+                v[u].load(vc + (uint32_t)(s * hs));
             }
-            acc = fmaf(acc, ks[s / a.block], rel);
-#pragma unroll
-            for (int k = 8; k > 0; k >>= 1) acc += __shfl_xor(acc, k, 64);
-            x[u] = t + u * GROUPS + grp < s1 ? acc * sc : -INFINITY;
         }
-        float mn = m;
+        float x[UN], mn = m;
 #pragma unroll
-        for (int u = 0; u < UN; ++u) mn = fmaxf(mn, x[u]);
-        const float f = pexp(m, mn);
-        m = mn;
-        l *= f;
+        for (int u = 0; u < UN; ++u) {
+            x[u] = dok ? fmaf(k[u].dot(q), fk[u], r[u].dot(q)) : 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] *= f;
+            for (int i = LPK / 2; i > 0; i >>= 1) x[u] += __shfl_xor(x[u], i, 64);
+            x[u] = t + u * GW + grp < n ? x[u] * sc : -INFINITY;
+            mn = fmaxf(mn, x[u]);
+        }
+        if (__any(mn > m)) {  // else the factor is 1
+            const float f = pexp(m, mn);
+            m = mn;
+            l *= f;
+#pragma unroll
+            for (int e = 0; e < VPL; ++e) o[e] *= f;
+        }
 #pragma unroll
         for (int u = 0; u < UN; ++u) {
             const float p = pexp(x[u], m);
-            const int s = min(t + u * GROUPS + grp, s1 - 1);
             l += p;
-            const float pv = p * vs[s / a.block];
-            if (t + u * GROUPS + grp < s1) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e) o[e] = fmaf(pv, v[u][e], o[e]);
-            }
+            if (dok && t + u * GW + grp < n) v[u].add_to(o, p * fv[u]);
         }
     }
-    // the 4 key groups of the wave
-    float M = fmaxf(m, __shfl_xor(m, 16, 64));
-    M = fmaxf(M, __shfl_xor(M, 32, 64));
+    // the key groups of the wave
+    float M = m;
+#pragma unroll
+    for (int i = LPK; i < 64; i <<= 1) M = fmaxf(M, __shfl_xor(M, i, 64));
     const float f = pexp(m, M);
     l *= f;
-    l += __shfl_xor(l, 16, 64);
-    l += __shfl_xor(l, 32, 64);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        o[e] *= f;
-        o[e] += __shfl_xor(o[e], 16, 64);
-        o[e] += __shfl_xor(o[e], 32, 64);
+    for (int e = 0; e < VPL; ++e) o[e] *= f;
+#pragma unroll
+    for (int i = LPK; i < 64; i <<= 1) {
+        l += __shfl_xor(l, i, 64);
+#pragma unroll
+        for (int e = 0; e < VPL; ++e) o[e] += __shfl_xor(o[e], i, 64);
     }
-    if (lane < 16 && dok) {
+    if (lane < LPK && dok) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) part[w][d0 + e] = o[e];
+        for (int e = 0; e < VPL; ++e) part[w][d0 + e] = o[e];
     }
     if (lane == 0) wm[w] = M, wl[w] = l;
     __syncthreads();
@@ -149,37 +239,66 @@ __global__ __launch_bounds__(NT) void decode_kv8_kernel(Args a) {
         return;
     }
     const int64_t pi = bh * a.nsplit + c;
-    if (tid < hs) a.po[pi * hs + tid] = acc;
-    if (tid == 0) a.pml[2 * pi] = M, a.pml[2 * pi + 1] = L;
+    if (n > 0 && tid < hs) a.po[pi * hs + tid] = acc;
+    if (tid == 0) a.pml[2 * pi] = M, a.pml[2 * pi + 1] = n > 0 ? L : -1.f;  // -1: no key in this chunk
 }
 
-// out[b, h] = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c over the chunks of the window
+// out[b, h] = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c over the chunks that hold keys
 template <typename T>
 __global__ __launch_bounds__(HS) void decode_kv8_join_kernel(Args a) {
     const int tid = threadIdx.x, h = blockIdx.x, hs = a.hs;
     const int64_t b = blockIdx.y, base = (b * a.H + h) * a.nsplit;
-    const int S = kv8_window(a.pos[b * a.pos_stride], a.n_meta, a.S_ring - a.n_meta);
-    const int nc = (S + a.chunk - 1) / a.chunk;
+    const f32x2* ml = (const f32x2*)a.pml + base;
     float M = -INFINITY;
-    for (int c = 0; c < nc; ++c) M = fmaxf(M, a.pml[2 * (base + c)]);
+    for (int c = 0; c < a.nsplit; ++c) M = fmaxf(M, ml[c][0]);  // an empty chunk's is -inf
     float L = 0.f, acc = 0.f;
-    for (int c = 0; c < nc; ++c) {
-        const float f = pexp(a.pml[2 * (base + c)], M);
-        L = fmaf(f, a.pml[2 * (base + c) + 1], L);
-        if (tid < hs) acc = fmaf(f, a.po[(base + c) * hs + tid], acc);
+    bool any = false;
+    for (int c = 0; c < a.nsplit; ++c) {
+        const f32x2 x = ml[c];
+        const float o = tid < hs ? a.po[(base + c) * hs + tid] : 0.f;  // not written where the chunk is empty
+        if (x[1] != -1.f) {
+            const float f = pexp(x[0], M);
+            L = fmaf(f, x[1], L);
+            acc = fmaf(f, o, acc);
+            any = true;
+        }
     }
-    if (tid < hs) ((T*)a.out)[b * a.ldo + (int64_t)h * hs + tid] = (T)(S > 0 ? acc / L : 0.f);
+    if (tid < hs) ((T*)a.out)[b * a.ldo + (int64_t)h * hs + tid] = (T)(any ? acc / L : 0.f);
 }
 
-// slots per workgroup: enough workgroups for the 256 CUs, whole steps of the loop
-int chunk_of(int64_t B, int64_t H, int64_t S_ring) {
-    const int64_t want = (S_ring * B * H + 2047) / 2048;
-    const int64_t c = (want + STEP - 1) / STEP * STEP;
-    return (int)std::min<int64_t>(c, (S_ring + STEP - 1) / STEP * STEP);
+// Chunks of a row's ring: enough workgroups for 256 CUs of four or more each, but
+// no chunk under 128 slots; whole multiples of 64 slots
+int64_t chunk_of(int64_t B, int64_t H, int64_t S_ring) {
+    const int64_t want = std::max<int64_t>(1, 4096 / (B * H));
+    const int64_t n = std::min(want, (S_ring + 127) / 128), c = (S_ring + n - 1) / n;
+    return (c + 63) / 64 * 64;
 }
 int64_t splits(int64_t B, int64_t H, int64_t S_ring) {
-    const int c = chunk_of(B, H, S_ring);
+    const int64_t c = chunk_of(B, H, S_ring);
     return (S_ring + c - 1) / c;
+}
+
+template <typename T, int VPL, int LPK>
+void launch_one(const Args& a, unsigned grid, hipStream_t s) {
+    hipLaunchKernelGGL((decode_kv8_kernel<T, VPL, LPK>), dim3(grid), dim3(NT), 0, s, a);
+}
+template <typename T>
+void launch(const Args& a, unsigned grid, hipStream_t s) {
+    // 16 codes per lane where the rows are 16-byte aligned
+    if (a.hs % 16 == 0 && (((uintptr_t)a.kc | (uintptr_t)a.vc) & 15) == 0) {
+        if (a.hs <= 16) launch_one<T, 16, 1>(a, grid, s);
+        else if (a.hs <= 32) launch_one<T, 16, 2>(a, grid, s);
+        else if (a.hs <= 64) launch_one<T, 16, 4>(a, grid, s);
+        else launch_one<T, 16, 8>(a, grid, s);
+    } else {
+        if (a.hs <= 8) launch_one<T, 8, 1>(a, grid, s);
+        else if (a.hs <= 16) launch_one<T, 8, 2>(a, grid, s);
+        else if (a.hs <= 32) launch_one<T, 8, 4>(a, grid, s);
+        else if (a.hs <= 64) launch_one<T, 8, 8>(a, grid, s);
+        else launch_one<T, 8, 16>(a, grid, s);
+    }
+    if (a.nsplit > 1)
+        hipLaunchKernelGGL(decode_kv8_join_kernel<T>, dim3((unsigned)a.H, (unsigned)a.B), dim3(HS), 0, s, a);
 }
 
 }  // namespace
@@ -214,22 +333,22 @@ extern "C" int msq_relattn_decode_kv8(int dtype, void* out, int64_t ldo, const v
     Args a;
     a.q = q; a.kc = (const uint8_t*)kc; a.vc = (const uint8_t*)vc; a.ks = ks; a.vs = vs; a.R = R; a.out = out;
     a.pos = pos; a.pos_stride = pos_stride; a.ldq = ldq; a.ldo = ldo; a.S_max = S_max;
-    a.H = (int)H; a.hs = (int)hs; a.S_ring = (int)S_ring; a.n_meta = (int)n_meta; a.block = (int)block;
+    a.B = (int)B; a.H = (int)H; a.hs = (int)hs; a.S_ring = (int)S_ring; a.n_meta = (int)n_meta;
+    a.block_log2 = __builtin_ctz((unsigned)block);
     a.nblk = (int)((S_ring + block - 1) / block);
-    a.chunk = chunk_of(B, H, S_ring);
+    a.chunk = (int)chunk_of(B, H, S_ring);
     a.nsplit = (int)splits(B, H, S_ring);
+    MSQ_CHECK_ARG((int64_t)a.chunk * hs < (1ll << 31), "%s: a ring of %lld for %lld x %lld heads", fn, (long long)S_ring,
+                  (long long)B, (long long)H);  // 32-bit offsets inside a chunk
     a.po = (float*)ws;
     a.pml = (float*)ws + B * H * a.nsplit * hs;
     a.scale = scale;
-    hipStream_t s = (hipStream_t)stream;
-    const dim3 grid((unsigned)a.nsplit, (unsigned)H, (unsigned)B), jgrid((unsigned)H, (unsigned)B);
-    if (dtype == MSQ_BF16) {
-        hipLaunchKernelGGL(decode_kv8_kernel<bf16>, grid, dim3(NT), 0, s, a);
-        if (a.nsplit > 1) hipLaunchKernelGGL(decode_kv8_join_kernel<bf16>, jgrid, dim3(HS), 0, s, a);
-    } else {
-        hipLaunchKernelGGL(decode_kv8_kernel<float>, grid, dim3(NT), 0, s, a);
-        if (a.nsplit > 1) hipLaunchKernelGGL(decode_kv8_join_kernel<float>, jgrid, dim3(HS), 0, s, a);
-    }
+    const int64_t pairs = H * a.nsplit;
+    a.remap = pairs >= 32;  // fewer would leave XCDs without work
+    const int64_t grid = (a.remap ? (pairs + 7) / 8 * 8 : pairs) * B;
+    MSQ_CHECK_ARG(grid < (1ll << 31), "%s: %lld workgroups", fn, (long long)grid);
+    if (dtype == MSQ_BF16) launch<bf16>(a, (unsigned)grid, (hipStream_t)stream);
+    else launch<float>(a, (unsigned)grid, (hipStream_t)stream);
     MSQ_LAUNCH_CHECK();
     return MSQ_OK;
 }
