@@ -9,14 +9,25 @@
 // Tokens outside [0, V) (padding) get lp = 0 and no gradient from g_y. The top
 // alternatives are ordered by value, equal ones by index; NaN counts as largest.
 //
-// One workgroup per row. A row whose address is not 16-byte aligned is read as
-// the aligned 16-byte vectors that cover it, the ones at its ends by element.
+// One workgroup per row. Forward: bound by the row's bytes, and close behind by
+// the VALU (some 12 operations an element at 13 that fit under 6 TB/s of bf16, the
+// exponential alone 4): the row is read once, into registers (up to 9 vectors of
+// 16 bytes a lane), the maximum taken first so that no running sum is rescaled.
+// Longer rows are streamed with a running maximum (and read a second time for
+// the top alternatives). A row whose address is not 16-byte aligned is read as the
+// aligned 16-byte vectors that cover it, the ones at its ends by element.
+//
+// Top k without sorting: the lanes are cut into K >= k sets (K a power of two); the
+// least of the sets' maxima is a bound that at least k elements reach and that
+// few do (about K (1 + 1/2 + .. + 1/K) for values in no order). Those are
+// listed in LDS and ranked by (value, index). A row of many equal values may list
+// more than fit; it is then searched k times (top_slow).
 #include "common.h"
 
 namespace {
 
 constexpr int MAXTOP = 32, CAP = 512;
-constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
+constexpr float LOG2E = 1.44269504088896340736f;
 
 template <typename T> struct Vec { static constexpr int N = 16 / sizeof(T); };
 
@@ -26,7 +37,7 @@ struct FwdArgs {
     const int64_t* tok;
     float *lp, *ent, *stats, *top_lp;
     int64_t* top_id;
-    int top;
+    int top, sets_log2;  // 2^sets_log2 >= top
 };
 
 template <typename T>
@@ -37,23 +48,32 @@ template <>
 __device__ __forceinline__ float elem<bf16>(u32x4 v, int e) {
     return __uint_as_float(e & 1 ? v[e >> 1] & 0xffff0000u : v[e >> 1] << 16);
 }
+template <typename T>
+__device__ __forceinline__ float vec_max(u32x4 v) {
+    float m = elem<T>(v, 0);
+#pragma unroll
+    for (int e = 1; e < Vec<T>::N; ++e) m = fmaxf(m, elem<T>(v, e));
+    return m;
+}
 
 // the row as aligned vectors: vector j holds elements j * N - off .. + N - 1
 template <typename T>
 struct Row {
+    static constexpr int N = Vec<T>::N;
     const T* x;
     int64_t V;
     int off;
     __device__ __forceinline__ Row(const void* base, int64_t row, int64_t ld, int64_t V_)
         : x((const T*)base + row * ld), V(V_), off((int)(((uintptr_t)x & 15) / sizeof(T))) {}
-    __device__ __forceinline__ int64_t vecs() const { return (V + off + Vec<T>::N - 1) / Vec<T>::N; }
+    __device__ __forceinline__ int64_t vecs() const { return (V + off + N - 1) / N; }
+    __device__ __forceinline__ int64_t at(int64_t j) const { return j * N - off; }
     // elements outside the row read as -inf
     __device__ __forceinline__ u32x4 load(int64_t j) const {
-        const int64_t i0 = j * Vec<T>::N - off;
-        if (i0 >= 0 && i0 + Vec<T>::N <= V) return *(const u32x4*)(x + i0);
-        union { u32x4 v; T t[Vec<T>::N]; } r;
+        const int64_t i0 = at(j);
+        if (i0 >= 0 && i0 + N <= V) return *(const u32x4*)(x + i0);
+        union { u32x4 v; T t[N]; } r;
 #pragma unroll
-        for (int e = 0; e < Vec<T>::N; ++e) r.t[e] = i0 + e >= 0 && i0 + e < V ? x[i0 + e] : (T)-INFINITY;
+        for (int e = 0; e < N; ++e) r.t[e] = i0 + e >= 0 && i0 + e < V ? x[i0 + e] : (T)-INFINITY;
         return r.v;
     }
 };
@@ -66,74 +86,44 @@ __device__ __forceinline__ uint32_t ordered(float x) {
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 __device__ __forceinline__ uint64_t key_of(float x, uint32_t i) { return (uint64_t)ordered(x) << 32 | (0xffffffffu - i); }
+__device__ __forceinline__ uint32_t key_index(uint64_t k) { return 0xffffffffu - (uint32_t)k; }
 
-template <int NT>
-__device__ __forceinline__ float block_sum(float v, float* red) {
-    v = wave_sum(v);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    float s = red[0];
-#pragma unroll
-    for (int i = 1; i < NT / 64; ++i) s += red[i];
-    return s;
-}
-template <int NT>
-__device__ __forceinline__ float block_max(float v, float* red) {
-    v = wave_max(v);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    float s = red[0];
-#pragma unroll
-    for (int i = 1; i < NT / 64; ++i) s = fmaxf(s, red[i]);
-    return s;
-}
-
-template <typename T, int NT>
-__global__ __launch_bounds__(NT) void token_logprobs_kernel(FwdArgs a) {
-    __shared__ float red[NT / 64];
-    __shared__ uint64_t kred[NT / 64];
-    const int tid = threadIdx.x;
-    const int64_t row = blockIdx.x;
-    const Row<T> R(a.x, row, a.ld, a.V);
-    const int64_t nv = R.vecs();
-    float m = -INFINITY;
-    for (int64_t j = tid; j < nv; j += NT) {
-        const u32x4 v = R.load(j);
-#pragma unroll
-        for (int e = 0; e < Vec<T>::N; ++e) m = fmaxf(m, elem<T>(v, e));
-    }
-    const float M = block_max<NT>(m, red), Mf = M == -INFINITY ? 0.f : M;
+// running sums of a row against the maximum m: s = sum e^(x - m), t = sum (x - m) e^(x - m)
+struct Sums {
     float s = 0.f, t = 0.f;
-    for (int64_t j = tid; j < nv; j += NT) {
-        const u32x4 v = R.load(j);
+    template <typename T>
+    __device__ __forceinline__ void add(u32x4 v, float m) {
 #pragma unroll
         for (int e = 0; e < Vec<T>::N; ++e) {
-            const float d = elem<T>(v, e) - Mf, p = __builtin_amdgcn_exp2f(d * LOG2E);
+            const float d = elem<T>(v, e) - m, p = __builtin_amdgcn_exp2f(d * LOG2E);
             s += p;
             t = fmaf(fmaxf(d, -1e30f), p, t);  // d = -inf: p = 0
         }
     }
-    s = block_sum<NT>(s, red);
-    t = block_sum<NT>(t, red);
-    const float ls = M == -INFINITY ? s : logf(s);  // no finite logit: 0, or NaN if one is
-    if (tid == 0) {
-        const int64_t y = a.tok[row];
-        a.lp[row] = y >= 0 && y < a.V ? (M == -INFINITY && s == 0.f ? -INFINITY : ((float)R.x[y] - M) - ls) : 0.f;
-        a.ent[row] = M == -INFINITY && s == 0.f ? 0.f : ls - t / s;
-        if (a.stats) a.stats[2 * row] = M, a.stats[2 * row + 1] = ls;
+    // to the maximum m + d, d >= 0 (or m = -inf: the sums are 0, or NaN)
+    __device__ __forceinline__ void rescale(float d) {
+        const float f = __builtin_amdgcn_exp2f(-d * LOG2E);
+        t = f * fmaf(-fminf(d, 1e30f), s, t);
+        s *= f;
     }
+};
+__device__ __forceinline__ float finite_or_0(float m) { return m == -INFINITY ? 0.f : m; }
+
+// The largest elements by repeated search (many equal values, or NaN)
+template <typename T, int NT>
+__device__ void top_slow(const Row<T>& R, int top, uint64_t* kred, uint64_t* out) {
+    const int tid = threadIdx.x;
+    const int64_t nv = R.vecs();
     uint64_t prev = ~0ull;
-    for (int k = 0; k < a.top; ++k) {  // the largest key below the one before
+    for (int k = 0; k < top; ++k) {  // the largest key below the one before
         uint64_t best = 0;
         for (int64_t j = tid; j < nv; j += NT) {
             const u32x4 v = R.load(j);
 #pragma unroll
             for (int e = 0; e < Vec<T>::N; ++e) {
-                const int64_t i = j * Vec<T>::N - R.off + e;
+                const int64_t i = R.at(j) + e;
                 const uint64_t key = key_of(elem<T>(v, e), (uint32_t)i);
-                if (i >= 0 && i < a.V && key < prev && key > best) best = key;
+                if (i >= 0 && i < R.V && key < prev && key > best) best = key;
             }
         }
 #pragma unroll
@@ -147,12 +137,131 @@ __global__ __launch_bounds__(NT) void token_logprobs_kernel(FwdArgs a) {
         best = kred[0];
 #pragma unroll
         for (int i = 1; i < NT / 64; ++i) best = kred[i] > best ? kred[i] : best;
-        prev = best;
-        if (tid == 0) {
-            const uint32_t i = 0xffffffffu - (uint32_t)best;
-            a.top_id[row * a.top + k] = i;
-            a.top_lp[row * a.top + k] = M == -INFINITY && s == 0.f ? -INFINITY : ((float)R.x[i] - M) - ls;
+        prev = best;  // top <= V: there is one
+        if (tid == 0) out[k] = best;
+    }
+    __syncthreads();
+}
+
+// NV > 0: the row in registers, NV vectors a lane; NV = 0: streamed
+template <typename T, int NT, int NV>
+__global__ __launch_bounds__(NT) void token_logprobs_kernel(FwdArgs a) {
+    constexpr int W = NT / 64, N = Vec<T>::N, NR = NV ? NV : 1, UN = 4;
+    __shared__ float lmax[NT], rs[W], rt[W];
+    __shared__ uint64_t list[CAP], best[MAXTOP];
+    __shared__ int count;
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    const int64_t row = blockIdx.x;
+    const Row<T> R(a.x, row, a.ld, a.V);
+    const int64_t nv = R.vecs();
+    int64_t y = 0;
+    float xy = 0.f;
+    if (tid == 0) {
+        count = 0;
+        y = a.tok[row];
+        if (y >= 0 && y < a.V) xy = (float)R.x[y];
+    }
+    u32x4 v[NR];
+    float vm[NR], m = -INFINITY;
+    Sums sum;
+    if constexpr (NV > 0) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int j = i * NT + tid;
+            v[i] = R.load(j);  // past the row: -inf throughout
         }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            vm[i] = vec_max<T>(v[i]);
+            m = fmaxf(m, vm[i]);
+        }
+    } else {
+        for (int64_t j = tid; j < nv; j += UN * NT) {
+            u32x4 u[UN];
+            float mn = m;
+#pragma unroll
+            for (int i = 0; i < UN; ++i) u[i] = R.load(j + i * NT);
+#pragma unroll
+            for (int i = 0; i < UN; ++i) mn = fmaxf(mn, vec_max<T>(u[i]));
+            const float mf = finite_or_0(mn);
+            sum.rescale(m == -INFINITY ? 0.f : mn - m);
+            m = mn;
+#pragma unroll
+            for (int i = 0; i < UN; ++i) sum.template add<T>(u[i], mf);
+        }
+    }
+    lmax[tid] = m;
+    __syncthreads();
+    // every wave: the maxima of 64 sets of lanes, the row's maximum, the bound for the top k
+    float g = lmax[lane];
+#pragma unroll
+    for (int i = 1; i < W; ++i) g = fmaxf(g, lmax[i * 64 + lane]);
+    float tau = -INFINITY;
+    for (int o = 32; o > 0; o >>= 1) {
+        if (o < 1 << a.sets_log2) {  // sets o apart in the lanes: from here on across them
+            if (o == (1 << a.sets_log2) >> 1) tau = g;
+            tau = fminf(tau, __shfl_xor(tau, o, 64));
+        }
+        g = fmaxf(g, __shfl_xor(g, o, 64));
+    }
+    if (a.sets_log2 == 0) tau = g;
+    const float M = g, Mf = finite_or_0(M);
+    auto push = [&](u32x4 u, int64_t j) {
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const float f = elem<T>(u, e);
+            const int64_t i = R.at(j) + e;
+            if (f >= tau && i >= 0 && i < a.V) {
+                const int at = atomicAdd(&count, 1);
+                if (at < CAP) list[at] = key_of(f, (uint32_t)i);
+            }
+        }
+    };
+    if constexpr (NV > 0) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) sum.template add<T>(v[i], Mf);
+        if (a.top)
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if (vm[i] >= tau) push(v[i], i * NT + tid);
+    } else {
+        sum.rescale(m == -INFINITY ? 0.f : M - m);
+        if (a.top && m >= tau)
+            for (int64_t j = tid; j < nv; j += NT) {
+                const u32x4 u = R.load(j);
+                if (vec_max<T>(u) >= tau) push(u, j);
+            }
+    }
+    const float ws = wave_sum(sum.s), wt = wave_sum(sum.t);
+    if (lane == 0) rs[w] = ws, rt[w] = wt;
+    __syncthreads();
+    float s = rs[0], t = rt[0];
+#pragma unroll
+    for (int i = 1; i < W; ++i) s += rs[i], t += rt[i];
+    const bool empty = M == -INFINITY && s == 0.f;   // no distribution
+    const float ls = M == -INFINITY ? s : logf(s);   // no finite logit: 0, or NaN if one is
+    if (tid == 0) {
+        a.lp[row] = y >= 0 && y < a.V ? (empty ? -INFINITY : (xy - M) - ls) : 0.f;
+        a.ent[row] = empty ? 0.f : ls - t / s;
+        if (a.stats) a.stats[2 * row] = M, a.stats[2 * row + 1] = ls;
+    }
+    if (!a.top) return;
+    const int n = count;
+    auto put = [&](int k, uint64_t key) {
+        const uint32_t i = key_index(key);
+        a.top_id[row * a.top + k] = i;
+        a.top_lp[row * a.top + k] = empty ? -INFINITY : ((float)R.x[i] - M) - ls;
+    };
+    if (n > CAP || s != s) {  // (uniform) too many for the list, or NaN, which no bound reaches
+        top_slow<T, NT>(R, a.top, list, best);
+        if (tid < a.top) put(tid, best[tid]);
+        return;
+    }
+    for (int c = tid; c < n; c += NT) {
+        const uint64_t key = list[c];
+        int rank = 0;
+        for (int i = 0; i < n; ++i) rank += list[i] > key;
+        if (rank < a.top) put(rank, key);
     }
 }
 
@@ -165,28 +274,109 @@ struct BwdArgs {
     int top;
 };
 
+template <typename T>
+__device__ __forceinline__ u32x4 pack(const float* d);
+template <>
+__device__ __forceinline__ u32x4 pack<float>(const float* d) {
+    return (u32x4){__float_as_uint(d[0]), __float_as_uint(d[1]), __float_as_uint(d[2]), __float_as_uint(d[3])};
+}
+template <>
+__device__ __forceinline__ u32x4 pack<bf16>(const float* d) {
+    union { bf16x8 b; u32x4 u; } r;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r.b[e] = (bf16)d[e];
+    return r.u;
+}
+
+// Streamed: read and written once, bound by that. The given token's and the
+// alternatives' elements are written again at the end, with their own terms.
 template <typename T, int NT>
 __global__ __launch_bounds__(NT) void token_logprobs_bwd_kernel(BwdArgs a) {
+    constexpr int N = Vec<T>::N, UN = 4;
     const int tid = threadIdx.x;
     const int64_t row = blockIdx.x;
     const Row<T> R(a.x, row, a.ld, a.V);
     T* dx = (T*)a.dx + row * a.ldd;
-    const float M = a.stats[2 * row], ls = a.stats[2 * row + 1];
-    const int64_t y = a.tok[row];
+    const bool same = (((uintptr_t)dx ^ (uintptr_t)R.x) & 15) == 0;  // both rows' vectors coincide
+    const float M = a.stats[2 * row], ls = a.stats[2 * row + 1], ls2 = ls * LOG2E;
+    const int64_t y = a.tok[row], nv = R.vecs();
     const float gy = a.g_lp && y >= 0 && y < a.V ? a.g_lp[row] : 0.f, gh = a.g_ent ? a.g_ent[row] : 0.f;
     float c = gy;
     if (a.g_top)
         for (int k = 0; k < a.top; ++k) c += a.g_top[row * a.top + k];
     c = -c - gh * a.ent[row];
     const bool empty = M == -INFINITY && ls == 0.f;
-    for (int64_t i = tid; i < a.V; i += NT) {
-        const float lp = ((float)R.x[i] - M) - ls, p = __builtin_amdgcn_exp2f(lp * LOG2E);
-        float d = p * fmaf(-gh, fmaxf(lp, -1e30f), c);
-        if (i == y) d += gy;
-        if (a.g_top)
-            for (int k = 0; k < a.top; ++k) d += a.top_id[row * a.top + k] == i ? a.g_top[row * a.top + k] : 0.f;
-        dx[i] = (T)(empty ? 0.f : d);
+    // p (c - g_H lp)
+    auto smooth = [&](float x) {
+        const float d = x - M, p = __builtin_amdgcn_exp2f(fmaf(d, LOG2E, -ls2));
+        return empty ? 0.f : p * fmaf(-gh, fmaxf(d - ls, -1e30f), c);
+    };
+    for (int64_t j0 = tid; j0 < nv; j0 += UN * NT) {
+        u32x4 v[UN];
+#pragma unroll
+        for (int u = 0; u < UN; ++u) v[u] = R.load(j0 + u * NT);
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+            float d[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) d[e] = smooth(elem<T>(v[u], e));
+            const int64_t i0 = R.at(j0 + u * NT);
+            if (same && i0 >= 0 && i0 + N <= a.V) {
+                *(u32x4*)(dx + i0) = pack<T>(d);
+            } else {
+#pragma unroll
+                for (int e = 0; e < N; ++e)
+                    if (i0 + e >= 0 && i0 + e < a.V) dx[i0 + e] = (T)d[e];
+            }
+        }
     }
+    __syncthreads();  // the rest overwrites elements that other lanes have written
+    const int picks = 1 + (a.g_top ? a.top : 0);
+    if (tid < picks) {
+        const int64_t i = tid == 0 ? y : a.top_id[row * a.top + tid - 1];
+        if (i >= 0 && i < a.V && !empty) {
+            float d = smooth((float)R.x[i]) + (i == y ? gy : 0.f);  // every pick of one element gives the same
+            for (int k = 0; k < picks - 1; ++k) d += a.top_id[row * a.top + k] == i ? a.g_top[row * a.top + k] : 0.f;
+            dx[i] = (T)d;
+        }
+    }
+}
+
+template <typename T>
+void launch_fwd(const FwdArgs& a, int64_t rows, hipStream_t s) {
+    const int64_t vecs = (a.V + 2 * (Vec<T>::N - 1)) / Vec<T>::N;  // whatever the row's alignment
+    const dim3 g((unsigned)rows);
+#define FWD(NT, NV)                                                                                      \
+    do {                                                                                                 \
+        if (vecs <= NT * NV) {                                                                           \
+            hipLaunchKernelGGL((token_logprobs_kernel<T, NT, NV>), g, dim3(NT), 0, s, a);                \
+            return;                                                                                      \
+        }                                                                                                \
+    } while (0)
+    // many rows: as few lanes a row as hold it, for many rows a CU; few: as many lanes as help
+    FWD(64, 1);
+    if (rows >= 1024) {
+        FWD(64, 3);
+        FWD(64, 9);
+        FWD(256, 5);
+        FWD(256, 9);
+    } else {
+        FWD(256, 1);
+    }
+    FWD(1024, 1);
+    FWD(1024, 3);
+    FWD(1024, 5);
+    FWD(1024, 9);
+#undef FWD
+    hipLaunchKernelGGL((token_logprobs_kernel<T, 1024, 0>), g, dim3(1024), 0, s, a);
+}
+template <typename T>
+void launch_bwd(const BwdArgs& a, int64_t rows, hipStream_t s) {
+    const int64_t vecs = a.V / Vec<T>::N;
+    const dim3 g((unsigned)rows);
+    if (vecs <= 256) hipLaunchKernelGGL((token_logprobs_bwd_kernel<T, 64>), g, dim3(64), 0, s, a);
+    else if (rows >= 1024) hipLaunchKernelGGL((token_logprobs_bwd_kernel<T, 256>), g, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((token_logprobs_bwd_kernel<T, 1024>), g, dim3(1024), 0, s, a);
 }
 
 }  // namespace
@@ -202,10 +392,10 @@ extern "C" int msq_token_logprobs(float* logprob, float* entropy, float* stats, 
     MSQ_CHECK_ARG(top >= 0 && top <= MAXTOP && top <= V, "%s: %lld alternatives of %lld (at most %d)", fn,
                   (long long)top, (long long)V, MAXTOP);
     MSQ_CHECK_ARG(top == 0 || (top_ids && top_logprobs), "%s: null pointer", fn);
-    const FwdArgs a{logits, ld, V, tokens, logprob, entropy, stats, top_logprobs, top_ids, (int)top};
-    hipStream_t s = (hipStream_t)stream;
-    if (dtype == MSQ_BF16) hipLaunchKernelGGL((token_logprobs_kernel<bf16, 256>), dim3((unsigned)rows), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((token_logprobs_kernel<float, 256>), dim3((unsigned)rows), dim3(256), 0, s, a);
+    FwdArgs a{logits, ld, V, tokens, logprob, entropy, stats, top_logprobs, top_ids, (int)top, 0};
+    while (1 << a.sets_log2 < top) ++a.sets_log2;
+    if (dtype == MSQ_BF16) launch_fwd<bf16>(a, rows, (hipStream_t)stream);
+    else launch_fwd<float>(a, rows, (hipStream_t)stream);
     MSQ_LAUNCH_CHECK();
     return MSQ_OK;
 }
@@ -223,10 +413,8 @@ extern "C" int msq_token_logprobs_bwd(void* dlogits, int64_t ldd, const float* g
     MSQ_CHECK_ARG(top >= 0 && top <= MAXTOP, "%s: %lld alternatives (at most %d)", fn, (long long)top, MAXTOP);
     MSQ_CHECK_ARG(!g_top || (top_ids && top > 0), "%s: the alternatives' gradient needs their ids", fn);
     const BwdArgs a{logits, dlogits, ld, ldd, V, tokens, top_ids, g_logprob, g_entropy, g_top, stats, entropy, (int)top};
-    hipStream_t s = (hipStream_t)stream;
-    if (dtype == MSQ_BF16)
-        hipLaunchKernelGGL((token_logprobs_bwd_kernel<bf16, 256>), dim3((unsigned)rows), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((token_logprobs_bwd_kernel<float, 256>), dim3((unsigned)rows), dim3(256), 0, s, a);
+    if (dtype == MSQ_BF16) launch_bwd<bf16>(a, rows, (hipStream_t)stream);
+    else launch_bwd<float>(a, rows, (hipStream_t)stream);
     MSQ_LAUNCH_CHECK();
     return MSQ_OK;
 }
