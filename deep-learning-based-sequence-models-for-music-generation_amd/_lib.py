@@ -174,12 +174,15 @@ def stream():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
-def on_current(dev):
-    """raises unless dev is the GPU whose current stream a launch would go to"""
-    if dev.type != "cuda":
+def stream_of(t):
+    """the current stream's handle for launches on tensor t, which has to be on the
+    current GPU"""
+    dev = t.get_device()
+    if dev < 0:
         raise RuntimeError("the MI355X kernels run on the GPU only (no CPU fallback)")
-    if dev.index != torch.cuda.current_device():
-        raise ValueError(f"tensors on {dev} while cuda:{torch.cuda.current_device()} is the current device")
+    if dev != torch.cuda.current_device():
+        raise ValueError(f"tensors on cuda:{dev} while cuda:{torch.cuda.current_device()} is the current device")
+    return torch._C._cuda_getCurrentRawStream(dev)  # current_stream(dev).cuda_stream without the object
 
 
 def dt(t):

@@ -3,7 +3,7 @@ models/transformer/model_transformer.py:41-90) over the libmidiseq C ABI."""
 import torch
 
 from . import _lib as L
-from ._lib import ptr, call, stream, dt, on_current
+from ._lib import ptr, call, stream, dt, stream_of
 from .ops import workspace
 
 N_META = 6  # metadata prefix (generate_matrix, model_transformer.py:14)
@@ -71,12 +71,13 @@ def kv8_cache(B, H, S_ring, hs, device="cuda", block=KV8_BLOCK, layers=()):
     return codes[0], scales[0], codes[1], scales[1]
 
 
-def _kv8_args(kc, ks, vc, vs, pos, n_meta, block, *others):
+def _kv8_args(kc, ks, vc, vs, pos, n_meta, block):
     """the checked cache: (pointers, (B, H, hs, S_ring, n_meta, block, pos, pos_stride))"""
-    if kc.dtype != torch.float8_e4m3fn or vc.dtype != kc.dtype or kc.dim() != 4 or kc.shape != vc.shape:
+    shape = kc.shape
+    if kc.dtype != torch.float8_e4m3fn or vc.dtype != torch.float8_e4m3fn or len(shape) != 4 or vc.shape != shape:
         raise ValueError(f"the cache is two float8_e4m3fn [B, H, S_ring, hs] tensors, got {kc.dtype} "
                          f"{tuple(kc.shape)} and {vc.dtype} {tuple(vc.shape)}")
-    B, H, S_ring, hs = kc.shape
+    B, H, S_ring, hs = shape
     if not 0 <= n_meta < S_ring or block not in (16, 32, 64, 128):
         raise ValueError(f"a ring of {S_ring} slots, {n_meta} of them metadata, in blocks of {block}")
     want = (B, H, -(-S_ring // block))
@@ -88,13 +89,21 @@ def _kv8_args(kc, ks, vc, vs, pos, n_meta, block, *others):
     n = pos.numel()
     if pos.dtype != torch.int64 or pos.dim() > 1 or (n != 1 and n != B) or not pos.is_contiguous():
         raise ValueError(f"pos is an int64 tensor of 1 or {B} positions, got {pos.dtype} {tuple(pos.shape)}")
-    dev = kc.device
-    for t in (vc, ks, vs, pos) + others:
-        if t.device != dev:
-            raise ValueError(f"tensors on {dev} and {t.device}")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in others):
-        raise ValueError("the 8-bit cache has no gradient: call it under torch.no_grad()")
-    return (ptr(kc), ptr(ks), ptr(vc), ptr(vs)), (B, H, hs, S_ring, n_meta, block, ptr(pos), 0 if n == 1 else 1)
+    dev = kc.get_device()
+    if vc.get_device() != dev or ks.get_device() != dev or vs.get_device() != dev or pos.get_device() != dev:
+        raise ValueError("the cache, its scales and pos have to be on one device")
+    return ((kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr()),
+            (B, H, hs, S_ring, n_meta, block, pos.data_ptr(), 0 if n == 1 else 1))
+
+
+def _kv8_beside(kc, *others):
+    """operands that go with the cache: on its device, without a gradient"""
+    grad = torch.is_grad_enabled()
+    for t in others:
+        if t.get_device() != kc.get_device():
+            raise ValueError(f"the cache is on {kc.device}, an operand on {t.device}")
+        if grad and t.requires_grad:
+            raise ValueError("the 8-bit cache has no gradient: call it under torch.no_grad()")
 
 
 def kv8_write(kc, ks, vc, vs, k, v, pos, *, n_meta=N_META, block=KV8_BLOCK):
@@ -102,20 +111,22 @@ def kv8_write(kc, ks, vc, vs, k, v, pos, *, n_meta=N_META, block=KV8_BLOCK):
     apart, any other strides, the same for both: e.g. views of a packed
     projection) at positions pos .. pos + T - 1 of the ring, in place
     (msq_kv8_write). pos: int64 [B], or [1] for all rows; -n_meta for a prompt
-    whose first n_meta rows are metadata; below that a row is left alone."""
-    if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.stride() != v.stride():
+    whose first n_meta rows are metadata; below that a row is left alone.
+    Positions are written in order."""
+    shape, strides = k.shape, k.stride()
+    if len(shape) != 4 or v.shape != shape or v.dtype != k.dtype or v.stride() != strides:
         raise ValueError(f"k and v are [B, T, H, hs] alike, got {k.dtype} {tuple(k.shape)} {k.stride()} and "
                          f"{v.dtype} {tuple(v.shape)} {v.stride()}")
-    cache, (B, H, hs, *rest) = _kv8_args(kc, ks, vc, vs, pos, n_meta, block, k, v)
-    T = k.shape[1]
-    if k.shape != (B, T, H, hs) or k.dtype not in (torch.float32, torch.bfloat16):
-        raise ValueError(f"{k.dtype} {tuple(k.shape)} rows for a cache of {B} x {H} heads of {hs}")
-    if (hs > 1 and k.stride(3) != 1) or (H > 1 and k.stride(2) != hs):
-        raise ValueError(f"a token's heads have to lie {hs} apart, got strides {k.stride()}")
-    on_current(kc.device)
-    if T == 0:
-        return
-    call("msq_kv8_write", dt(k), *cache, ptr(k), ptr(v), k.stride(0), k.stride(1), B, T, H, hs, *rest, stream())
+    cache, (B, H, hs, *rest) = _kv8_args(kc, ks, vc, vs, pos, n_meta, block)
+    _kv8_beside(kc, k, v)
+    T = shape[1]
+    if shape != (B, T, H, hs) or k.dtype not in (torch.float32, torch.bfloat16):
+        raise ValueError(f"{k.dtype} {tuple(shape)} rows for a cache of {B} x {H} heads of {hs}")
+    if strides[3] != 1 or (H > 1 and strides[2] != hs):
+        raise ValueError(f"a token's heads have to lie {hs} apart, got strides {strides}")
+    s = stream_of(kc)
+    if T and B and H:
+        call("msq_kv8_write", dt(k), *cache, k.data_ptr(), v.data_ptr(), strides[0], strides[1], B, T, H, hs, *rest, s)
 
 
 def kv8_read(kc, ks, vc, vs, pos, *, first=0, rows=None, dtype=torch.bfloat16, n_meta=N_META, block=KV8_BLOCK):
@@ -126,11 +137,11 @@ def kv8_read(kc, ks, vc, vs, pos, *, first=0, rows=None, dtype=torch.bfloat16, n
     rows = S_ring - first if rows is None else rows
     if first < 0 or rows < 0 or first + rows > S_ring or dtype not in (torch.float32, torch.bfloat16):
         raise ValueError(f"rows {first} .. {first + rows} of a ring of {S_ring} in {dtype}")
-    on_current(kc.device)
-    k = torch.empty(B, H, rows, hs, device=kc.device, dtype=dtype)
+    s = stream_of(kc)
+    k = torch.empty((B, H, rows, hs), device=kc.device, dtype=dtype)
     v = torch.empty_like(k)
-    if rows:
-        call("msq_kv8_read", dt(k), ptr(k), ptr(v), *cache, B, H, hs, S_ring, *rest, first, rows, stream())
+    if rows and B and H:
+        call("msq_kv8_read", dt(k), k.data_ptr(), v.data_ptr(), *cache, B, H, hs, S_ring, *rest, first, rows, s)
     return k, v
 
 
@@ -139,25 +150,33 @@ def relattn_decode_kv8(q, kc, ks, vc, vs, R, pos, scale, *, out=None, n_meta=N_M
     newest position is pos (msq_relattn_decode_kv8): q [B, H, hs] (heads hs
     apart), R [H, S_max, hs] contiguous, both fp32 or bf16. Returns out [B, H,
     hs] in that type; rows that are not in use (pos < -n_meta) get zeros."""
-    if q.dim() != 3 or q.dtype not in (torch.float32, torch.bfloat16) or R.dtype != q.dtype:
+    if len(q.shape) != 3 or q.dtype not in (torch.float32, torch.bfloat16) or R.dtype != q.dtype:
         raise ValueError(f"q [B, H, hs] and R in fp32 or bf16, got {q.dtype} {tuple(q.shape)} and {R.dtype}")
+    cache, (B, H, hs, S_ring, *rest) = _kv8_args(kc, ks, vc, vs, pos, n_meta, block)
+    _kv8_beside(kc, q, R)
+    S_max = R.shape[1] if len(R.shape) == 3 else 0
+    if q.shape != (B, H, hs) or S_max < S_ring or R.shape != (H, S_max, hs) or not R.is_contiguous():
+        raise ValueError(f"q {tuple(q.shape)} and R {tuple(R.shape)} (contiguous: {R.is_contiguous()}) for a cache of "
+                         f"{B} x {H} x {S_ring} x {hs}")
+    sq = q.stride()
     if out is None:
-        out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-    cache, (B, H, hs, S_ring, *rest) = _kv8_args(kc, ks, vc, vs, pos, n_meta, block, q, R, out)
-    if q.shape != (B, H, hs) or R.dim() != 3 or R.shape[0] != H or R.shape[1] < S_ring or R.shape[2] != hs:
-        raise ValueError(f"q {tuple(q.shape)} and R {tuple(R.shape)} for a cache of {B} x {H} x {S_ring} x {hs}")
-    if out.shape != q.shape or out.dtype != q.dtype:
-        raise ValueError(f"out {out.dtype} {tuple(out.shape)} for q {q.dtype} {tuple(q.shape)}")
-    for t in (q, out):
-        if (hs > 1 and t.stride(2) != 1) or (H > 1 and t.stride(1) != hs):
-            raise ValueError(f"a row's heads have to lie {hs} apart, got strides {t.stride()}")
-    if not R.is_contiguous():
-        raise ValueError("R has to be contiguous")
-    on_current(kc.device)
+        so = (H * hs, hs, 1)
+    else:
+        _kv8_beside(kc, out)
+        so = out.stride()
+        if out.shape != q.shape or out.dtype != q.dtype:
+            raise ValueError(f"out {out.dtype} {tuple(out.shape)} for q {q.dtype} {tuple(q.shape)}")
+    if sq[2] != 1 or so[2] != 1 or (H > 1 and (sq[1] != hs or so[1] != hs)):
+        raise ValueError(f"a row's heads have to lie {hs} apart, got strides {sq} and {so}")
+    s = stream_of(kc)
+    if out is None:
+        out = torch.empty((B, H, hs), device=q.device, dtype=q.dtype)
+    if B == 0 or H == 0:
+        return out
     n = L.lib().msq_relattn_decode_kv8_workspace(B, H, hs, S_ring)
     # a scratch of its own for every call: captured graphs and streams never share one
     ws = torch.empty(n, device=q.device, dtype=torch.uint8) if n else None
-    call("msq_relattn_decode_kv8", dt(q), ptr(out), out.stride(0) if B > 1 else H * hs, ptr(q),
-         q.stride(0) if B > 1 else H * hs, *cache, ptr(R), R.shape[1], B, H, hs, S_ring, *rest, float(scale), ptr(ws), n,
-         stream())
+    call("msq_relattn_decode_kv8", dt(q), out.data_ptr(), so[0] if B > 1 else H * hs, q.data_ptr(),
+         sq[0] if B > 1 else H * hs, *cache, R.data_ptr(), S_max, B, H, hs, S_ring, *rest, float(scale),
+         ws.data_ptr() if n else None, n, s)
     return out

@@ -17,16 +17,17 @@
 // the top alternatives). A row whose address is not 16-byte aligned is read as the
 // aligned 16-byte vectors that cover it, the ones at its ends by element.
 //
-// Top k without sorting: the lanes are cut into K >= k sets (K a power of two); the
-// least of the sets' maxima is a bound that at least k elements reach and that
-// few do (about K (1 + 1/2 + .. + 1/K) for values in no order). Those are
-// listed in LDS and ranked by (value, index). A row of many equal values may list
-// more than fit; it is then searched k times (top_slow).
+// Top k without sorting: of the maxima of 64 sets of lanes the k-th largest is a
+// bound that at least k elements reach and hardly more do (k (1 + k / 128) or so
+// for values in no order). It is found by bisection over the upper 16 bits of the
+// values' order, with a ballot a bit. The vectors that hold such elements are
+// listed in LDS, the elements ranked by (value, index). A row of many equal
+// values may list more than fit; it is then searched k times (top_slow).
 #include "common.h"
 
 namespace {
 
-constexpr int MAXTOP = 32, CAP = 512;
+constexpr int MAXTOP = 32, VCAP = 128, CAP = 128;
 constexpr float LOG2E = 1.44269504088896340736f;
 
 template <typename T> struct Vec { static constexpr int N = 16 / sizeof(T); };
@@ -37,8 +38,22 @@ struct FwdArgs {
     const int64_t* tok;
     float *lp, *ent, *stats, *top_lp;
     int64_t* top_id;
-    int top, sets_log2;  // 2^sets_log2 >= top
+    int64_t rows;
+    int top;
 };
+
+// A row of one wave needs no barrier: LDS operations of a wave are in order. Such
+// rows go four to a workgroup.
+template <int NT>
+__device__ __forceinline__ void row_sync() {
+    if constexpr (NT > 64) {
+        __syncthreads();
+    } else {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+constexpr int rows_per_block(int NT) { return NT == 64 ? 4 : 1; }
 
 template <typename T>
 __device__ __forceinline__ float elem(u32x4 v, int e);
@@ -88,6 +103,19 @@ __device__ __forceinline__ uint32_t ordered(float x) {
 __device__ __forceinline__ uint64_t key_of(float x, uint32_t i) { return (uint64_t)ordered(x) << 32 | (0xffffffffu - i); }
 __device__ __forceinline__ uint32_t key_index(uint64_t k) { return 0xffffffffu - (uint32_t)k; }
 
+// a value that at least k of the wave's 64 values g reach and no more than about k do
+__device__ __forceinline__ float kth_bound(float g, int k) {
+    const uint32_t o = ordered(g);
+    uint32_t t = 0;
+#pragma unroll
+    for (int bit = 31; bit >= 16; --bit) {
+        const uint32_t c = t | 1u << bit;
+        if (__popcll(__ballot(o >= c)) >= k) t = c;  // (uniform)
+    }
+    // the value of that order; -inf where fewer than k sets hold a finite one
+    return t <= ordered(-INFINITY) ? -INFINITY : __uint_as_float(t & 0x80000000u ? t ^ 0x80000000u : ~t);
+}
+
 // running sums of a row against the maximum m: s = sum e^(x - m), t = sum (x - m) e^(x - m)
 struct Sums {
     float s = 0.f, t = 0.f;
@@ -112,7 +140,7 @@ __device__ __forceinline__ float finite_or_0(float m) { return m == -INFINITY ? 
 // The largest elements by repeated search (many equal values, or NaN)
 template <typename T, int NT>
 __device__ void top_slow(const Row<T>& R, int top, uint64_t* kred, uint64_t* out) {
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x % NT;
     const int64_t nv = R.vecs();
     uint64_t prev = ~0ull;
     for (int k = 0; k < top; ++k) {  // the largest key below the one before
@@ -131,48 +159,54 @@ __device__ void top_slow(const Row<T>& R, int top, uint64_t* kred, uint64_t* out
             const uint64_t other = __shfl_xor((unsigned long long)best, o, 64);
             best = other > best ? other : best;
         }
-        __syncthreads();
+        row_sync<NT>();
         if ((tid & 63) == 0) kred[tid >> 6] = best;
-        __syncthreads();
+        row_sync<NT>();
         best = kred[0];
 #pragma unroll
         for (int i = 1; i < NT / 64; ++i) best = kred[i] > best ? kred[i] : best;
         prev = best;  // top <= V: there is one
         if (tid == 0) out[k] = best;
     }
-    __syncthreads();
+    row_sync<NT>();
 }
 
 // NV > 0: the row in registers, NV vectors a lane; NV = 0: streamed
 template <typename T, int NT, int NV>
-__global__ __launch_bounds__(NT) void token_logprobs_kernel(FwdArgs a) {
-    constexpr int W = NT / 64, N = Vec<T>::N, NR = NV ? NV : 1, UN = 4;
-    __shared__ float lmax[NT], rs[W], rt[W];
-    __shared__ uint64_t list[CAP], best[MAXTOP];
-    __shared__ int count;
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    const int64_t row = blockIdx.x;
+__global__ __launch_bounds__(NT * rows_per_block(NT)) void token_logprobs_kernel(FwdArgs a) {
+    constexpr int W = NT / 64, N = Vec<T>::N, NR = NV ? NV : 1, UN = 4, RB = rows_per_block(NT);
+    __shared__ float lmax_[RB][NT], rs_[RB][W], rt_[RB][W];
+    __shared__ u32x4 vecs_[RB][VCAP];
+    __shared__ uint32_t vec_at_[RB][VCAP];
+    __shared__ uint64_t list_[RB][CAP], best_[RB][MAXTOP];
+    __shared__ int count_[RB][2];
+    const int tid = threadIdx.x % NT, lane = tid & 63, w = tid >> 6, sub = threadIdx.x / NT;
+    const int64_t row = (int64_t)blockIdx.x * RB + sub;
+    if (RB > 1 && row >= a.rows) return;
+    float *lmax = lmax_[sub], *rs = rs_[sub], *rt = rt_[sub];
+    int* count = count_[sub];
     const Row<T> R(a.x, row, a.ld, a.V);
     const int64_t nv = R.vecs();
     int64_t y = 0;
     float xy = 0.f;
     if (tid == 0) {
-        count = 0;
+        count[0] = count[1] = 0;
         y = a.tok[row];
         if (y >= 0 && y < a.V) xy = (float)R.x[y];
     }
+    // whether this wave's i-th vectors hold any of the row (uniform)
+    auto live = [&](int i) { return i * NT + w * 64 < nv; };
     u32x4 v[NR];
     float vm[NR], m = -INFINITY;
     Sums sum;
     if constexpr (NV > 0) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int j = i * NT + tid;
-            v[i] = R.load(j);  // past the row: -inf throughout
-        }
+        for (int i = 0; i < NV; ++i)
+            if (live(i)) v[i] = R.load(i * NT + tid);  // past the row: -inf throughout
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            vm[i] = vec_max<T>(v[i]);
+            vm[i] = -INFINITY;
+            if (live(i)) vm[i] = vec_max<T>(v[i]);
             m = fmaxf(m, vm[i]);
         }
     } else {
@@ -190,40 +224,30 @@ __global__ __launch_bounds__(NT) void token_logprobs_kernel(FwdArgs a) {
             for (int i = 0; i < UN; ++i) sum.template add<T>(u[i], mf);
         }
     }
-    lmax[tid] = m;
-    __syncthreads();
-    // every wave: the maxima of 64 sets of lanes, the row's maximum, the bound for the top k
-    float g = lmax[lane];
+    float g = m;
+    if constexpr (W > 1) {
+        lmax[tid] = m;
+        row_sync<NT>();
+        g = lmax[lane];
 #pragma unroll
-    for (int i = 1; i < W; ++i) g = fmaxf(g, lmax[i * 64 + lane]);
-    float tau = -INFINITY;
-    for (int o = 32; o > 0; o >>= 1) {
-        if (o < 1 << a.sets_log2) {  // sets o apart in the lanes: from here on across them
-            if (o == (1 << a.sets_log2) >> 1) tau = g;
-            tau = fminf(tau, __shfl_xor(tau, o, 64));
-        }
-        g = fmaxf(g, __shfl_xor(g, o, 64));
+        for (int i = 1; i < W; ++i) g = fmaxf(g, lmax[i * 64 + lane]);
     }
-    if (a.sets_log2 == 0) tau = g;
+    // every wave: from the maxima of 64 sets of lanes the row's maximum and the bound for the top k
+    const float tau = a.top ? kth_bound(g, a.top) : 0.f;
+    g = wave_max(g);
     const float M = g, Mf = finite_or_0(M);
     auto push = [&](u32x4 u, int64_t j) {
-#pragma unroll
-        for (int e = 0; e < N; ++e) {
-            const float f = elem<T>(u, e);
-            const int64_t i = R.at(j) + e;
-            if (f >= tau && i >= 0 && i < a.V) {
-                const int at = atomicAdd(&count, 1);
-                if (at < CAP) list[at] = key_of(f, (uint32_t)i);
-            }
-        }
+        const int at = atomicAdd(&count[0], 1);
+        if (at < VCAP) vecs_[sub][at] = u, vec_at_[sub][at] = (uint32_t)j;
     };
     if constexpr (NV > 0) {
 #pragma unroll
-        for (int i = 0; i < NV; ++i) sum.template add<T>(v[i], Mf);
+        for (int i = 0; i < NV; ++i)
+            if (live(i)) sum.template add<T>(v[i], Mf);
         if (a.top)
 #pragma unroll
             for (int i = 0; i < NV; ++i)
-                if (vm[i] >= tau) push(v[i], i * NT + tid);
+                if (live(i) && vm[i] >= tau) push(v[i], i * NT + tid);
     } else {
         sum.rescale(m == -INFINITY ? 0.f : M - m);
         if (a.top && m >= tau)
@@ -232,12 +256,14 @@ __global__ __launch_bounds__(NT) void token_logprobs_kernel(FwdArgs a) {
                 if (vec_max<T>(u) >= tau) push(u, j);
             }
     }
-    const float ws = wave_sum(sum.s), wt = wave_sum(sum.t);
-    if (lane == 0) rs[w] = ws, rt[w] = wt;
-    __syncthreads();
-    float s = rs[0], t = rt[0];
+    float s = wave_sum(sum.s), t = wave_sum(sum.t);
+    if constexpr (W > 1) {
+        if (lane == 0) rs[w] = s, rt[w] = t;
+        row_sync<NT>();
+        s = rs[0], t = rt[0];
 #pragma unroll
-    for (int i = 1; i < W; ++i) s += rs[i], t += rt[i];
+        for (int i = 1; i < W; ++i) s += rs[i], t += rt[i];
+    }
     const bool empty = M == -INFINITY && s == 0.f;   // no distribution
     const float ls = M == -INFINITY ? s : logf(s);   // no finite logit: 0, or NaN if one is
     if (tid == 0) {
@@ -246,15 +272,30 @@ __global__ __launch_bounds__(NT) void token_logprobs_kernel(FwdArgs a) {
         if (a.stats) a.stats[2 * row] = M, a.stats[2 * row + 1] = ls;
     }
     if (!a.top) return;
-    const int n = count;
+    if constexpr (W == 1) row_sync<NT>();
+    uint64_t* list = list_[sub];
     auto put = [&](int k, uint64_t key) {
         const uint32_t i = key_index(key);
         a.top_id[row * a.top + k] = i;
         a.top_lp[row * a.top + k] = empty ? -INFINITY : ((float)R.x[i] - M) - ls;
     };
-    if (n > CAP || s != s) {  // (uniform) too many for the list, or NaN, which no bound reaches
-        top_slow<T, NT>(R, a.top, list, best);
-        if (tid < a.top) put(tid, best[tid]);
+    // the listed vectors' elements that reach the bound
+    const int nvec = min(count[0], VCAP + 1);
+    if (nvec <= VCAP) {
+        for (int c = tid; c < nvec * N; c += NT) {
+            const float f = elem<T>(vecs_[sub][c / N], c % N);
+            const int64_t i = R.at(vec_at_[sub][c / N]) + c % N;
+            if (f >= tau && i >= 0 && i < a.V) {
+                const int at = atomicAdd(&count[1], 1);
+                if (at < CAP) list[at] = key_of(f, (uint32_t)i);
+            }
+        }
+    }
+    row_sync<NT>();
+    const int n = count[1];
+    if (nvec > VCAP || n > CAP || s != s) {  // (uniform) too many for the lists, or NaN, which no bound reaches
+        top_slow<T, NT>(R, a.top, list, best_[sub]);
+        if (tid < a.top) put(tid, best_[sub][tid]);
         return;
     }
     for (int c = tid; c < n; c += NT) {
@@ -271,6 +312,7 @@ struct BwdArgs {
     int64_t ld, ldd, V;
     const int64_t *tok, *top_id;
     const float *g_lp, *g_ent, *g_top, *stats, *ent;
+    int64_t rows;
     int top;
 };
 
@@ -291,10 +333,11 @@ __device__ __forceinline__ u32x4 pack<bf16>(const float* d) {
 // Streamed: read and written once, bound by that. The given token's and the
 // alternatives' elements are written again at the end, with their own terms.
 template <typename T, int NT>
-__global__ __launch_bounds__(NT) void token_logprobs_bwd_kernel(BwdArgs a) {
-    constexpr int N = Vec<T>::N, UN = 4;
-    const int tid = threadIdx.x;
-    const int64_t row = blockIdx.x;
+__global__ __launch_bounds__(NT * rows_per_block(NT)) void token_logprobs_bwd_kernel(BwdArgs a) {
+    constexpr int N = Vec<T>::N, UN = 4, RB = rows_per_block(NT);
+    const int tid = threadIdx.x % NT, w0 = tid & ~63;
+    const int64_t row = (int64_t)blockIdx.x * RB + threadIdx.x / NT;
+    if (RB > 1 && row >= a.rows) return;
     const Row<T> R(a.x, row, a.ld, a.V);
     T* dx = (T*)a.dx + row * a.ldd;
     const bool same = (((uintptr_t)dx ^ (uintptr_t)R.x) & 15) == 0;  // both rows' vectors coincide
@@ -311,12 +354,16 @@ __global__ __launch_bounds__(NT) void token_logprobs_bwd_kernel(BwdArgs a) {
         const float d = x - M, p = __builtin_amdgcn_exp2f(fmaf(d, LOG2E, -ls2));
         return empty ? 0.f : p * fmaf(-gh, fmaxf(d - ls, -1e30f), c);
     };
-    for (int64_t j0 = tid; j0 < nv; j0 += UN * NT) {
+    for (int64_t j1 = 0; j1 < nv; j1 += UN * NT) {
+        const int64_t j0 = j1 + tid;
         u32x4 v[UN];
+        auto live = [&](int u) { return j1 + u * NT + w0 < nv; };  // (uniform over the wave)
 #pragma unroll
-        for (int u = 0; u < UN; ++u) v[u] = R.load(j0 + u * NT);
+        for (int u = 0; u < UN; ++u)
+            if (live(u)) v[u] = R.load(j0 + u * NT);
 #pragma unroll
         for (int u = 0; u < UN; ++u) {
+            if (!live(u)) break;
             float d[N];
 #pragma unroll
             for (int e = 0; e < N; ++e) d[e] = smooth(elem<T>(v[u], e));
@@ -330,7 +377,9 @@ __global__ __launch_bounds__(NT) void token_logprobs_bwd_kernel(BwdArgs a) {
             }
         }
     }
-    __syncthreads();  // the rest overwrites elements that other lanes have written
+    // the rest overwrites elements that other lanes have written: their stores first
+    if constexpr (NT > 64) __syncthreads();
+    else __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup"), __builtin_amdgcn_wave_barrier();
     const int picks = 1 + (a.g_top ? a.top : 0);
     if (tid < picks) {
         const int64_t i = tid == 0 ? y : a.top_id[row * a.top + tid - 1];
@@ -345,11 +394,12 @@ __global__ __launch_bounds__(NT) void token_logprobs_bwd_kernel(BwdArgs a) {
 template <typename T>
 void launch_fwd(const FwdArgs& a, int64_t rows, hipStream_t s) {
     const int64_t vecs = (a.V + 2 * (Vec<T>::N - 1)) / Vec<T>::N;  // whatever the row's alignment
-    const dim3 g((unsigned)rows);
 #define FWD(NT, NV)                                                                                      \
     do {                                                                                                 \
         if (vecs <= NT * NV) {                                                                           \
-            hipLaunchKernelGGL((token_logprobs_kernel<T, NT, NV>), g, dim3(NT), 0, s, a);                \
+            constexpr int RB = rows_per_block(NT);                                                       \
+            hipLaunchKernelGGL((token_logprobs_kernel<T, NT, NV>), dim3((unsigned)((rows + RB - 1) / RB)), \
+                               dim3(NT * RB), 0, s, a);                                                  \
             return;                                                                                      \
         }                                                                                                \
     } while (0)
@@ -360,6 +410,7 @@ void launch_fwd(const FwdArgs& a, int64_t rows, hipStream_t s) {
         FWD(64, 9);
         FWD(256, 5);
         FWD(256, 9);
+        FWD(512, 9);
     } else {
         FWD(256, 1);
     }
@@ -368,13 +419,14 @@ void launch_fwd(const FwdArgs& a, int64_t rows, hipStream_t s) {
     FWD(1024, 5);
     FWD(1024, 9);
 #undef FWD
-    hipLaunchKernelGGL((token_logprobs_kernel<T, 1024, 0>), g, dim3(1024), 0, s, a);
+    hipLaunchKernelGGL((token_logprobs_kernel<T, 1024, 0>), dim3((unsigned)rows), dim3(1024), 0, s, a);
 }
 template <typename T>
 void launch_bwd(const BwdArgs& a, int64_t rows, hipStream_t s) {
     const int64_t vecs = a.V / Vec<T>::N;
     const dim3 g((unsigned)rows);
-    if (vecs <= 256) hipLaunchKernelGGL((token_logprobs_bwd_kernel<T, 64>), g, dim3(64), 0, s, a);
+    if (vecs <= 256)
+        hipLaunchKernelGGL((token_logprobs_bwd_kernel<T, 64>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
     else if (rows >= 1024) hipLaunchKernelGGL((token_logprobs_bwd_kernel<T, 256>), g, dim3(256), 0, s, a);
     else hipLaunchKernelGGL((token_logprobs_bwd_kernel<T, 1024>), g, dim3(1024), 0, s, a);
 }
@@ -392,8 +444,7 @@ extern "C" int msq_token_logprobs(float* logprob, float* entropy, float* stats, 
     MSQ_CHECK_ARG(top >= 0 && top <= MAXTOP && top <= V, "%s: %lld alternatives of %lld (at most %d)", fn,
                   (long long)top, (long long)V, MAXTOP);
     MSQ_CHECK_ARG(top == 0 || (top_ids && top_logprobs), "%s: null pointer", fn);
-    FwdArgs a{logits, ld, V, tokens, logprob, entropy, stats, top_logprobs, top_ids, (int)top, 0};
-    while (1 << a.sets_log2 < top) ++a.sets_log2;
+    const FwdArgs a{logits, ld, V, tokens, logprob, entropy, stats, top_logprobs, top_ids, rows, (int)top};
     if (dtype == MSQ_BF16) launch_fwd<bf16>(a, rows, (hipStream_t)stream);
     else launch_fwd<float>(a, rows, (hipStream_t)stream);
     MSQ_LAUNCH_CHECK();
@@ -412,7 +463,7 @@ extern "C" int msq_token_logprobs_bwd(void* dlogits, int64_t ldd, const float* g
                   (long long)ld, (long long)ldd);
     MSQ_CHECK_ARG(top >= 0 && top <= MAXTOP, "%s: %lld alternatives (at most %d)", fn, (long long)top, MAXTOP);
     MSQ_CHECK_ARG(!g_top || (top_ids && top > 0), "%s: the alternatives' gradient needs their ids", fn);
-    const BwdArgs a{logits, dlogits, ld, ldd, V, tokens, top_ids, g_logprob, g_entropy, g_top, stats, entropy, (int)top};
+    const BwdArgs a{logits, dlogits, ld, ldd, V, tokens, top_ids, g_logprob, g_entropy, g_top, stats, entropy, rows, (int)top};
     if (dtype == MSQ_BF16) launch_bwd<bf16>(a, rows, (hipStream_t)stream);
     else launch_bwd<float>(a, rows, (hipStream_t)stream);
     MSQ_LAUNCH_CHECK();

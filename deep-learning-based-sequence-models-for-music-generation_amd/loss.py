@@ -17,7 +17,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib as L
-from ._lib import ptr, call, stream, dt, on_current
+from ._lib import ptr, call, stream, dt, stream_of
 from .config import Grammar
 from .ops import workspace
 
@@ -148,24 +148,31 @@ class TokenLogprobs(NamedTuple):
     top_logprobs: Optional[torch.Tensor]   # fp32 [..., top]
 
 
+def _token_logprobs(x, tokens, top, stats):
+    """the launch on rows x [rows, V]; results in the tokens' shape"""
+    lp = torch.empty(tokens.shape, device=x.device, dtype=torch.float32)
+    ent = torch.empty_like(lp)
+    ids = top_lp = None
+    if top:
+        ids = torch.empty(tokens.shape + (top,), device=x.device, dtype=torch.int64)
+        top_lp = torch.empty_like(ids, dtype=torch.float32)
+    rows, V = x.shape
+    call("msq_token_logprobs", lp.data_ptr(), ent.data_ptr(), stats.data_ptr() if stats is not None else None,
+         ids.data_ptr() if top else None, top_lp.data_ptr() if top else None, x.data_ptr(), dt(x), x.stride(0),
+         tokens.data_ptr(), rows, V, top, stream_of(x))
+    return lp, ent, ids, top_lp
+
+
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, tokens, top):
-        rows, V = x.shape
-        f32 = dict(device=x.device, dtype=torch.float32)
-        lp, ent = torch.empty(rows, **f32), torch.empty(rows, **f32)
-        need = ctx.needs_input_grad[0]
-        stats = torch.empty(rows, 2, **f32) if need else None
-        ids = torch.empty(rows, top, device=x.device, dtype=torch.int64) if top else None
-        top_lp = torch.empty(rows, top, **f32) if top else None
-        call("msq_token_logprobs", ptr(lp), ptr(ent), ptr(stats), ptr(ids), ptr(top_lp), ptr(x), dt(x), x.stride(0),
-             ptr(tokens), rows, V, top, stream())
-        if need:
-            ctx.save_for_backward(x, tokens, stats, ent, ids)
-            ctx.top = top
-            ctx.set_materialize_grads(False)
-            if top:
-                ctx.mark_non_differentiable(ids)
+        stats = torch.empty(x.shape[0], 2, device=x.device, dtype=torch.float32)
+        lp, ent, ids, top_lp = _token_logprobs(x, tokens, top, stats)
+        ctx.save_for_backward(x, tokens, stats, ent, ids)
+        ctx.top = top
+        ctx.set_materialize_grads(False)
+        if top:
+            ctx.mark_non_differentiable(ids)
         return lp, ent, ids, top_lp
 
     @staticmethod
@@ -181,7 +188,7 @@ class _TokenLogprobs(torch.autograd.Function):
         dx = torch.empty(rows, ld, device=x.device, dtype=x.dtype)[:, :V]
         g = [None if t is None else t.to(torch.float32).contiguous() for t in (g_lp, g_ent, g_top)]
         call("msq_token_logprobs_bwd", ptr(dx), ld, ptr(g[0]), ptr(g[1]), ptr(g[2]), ptr(stats), ptr(ent), ptr(ids),
-             ctx.top, ptr(x), dt(x), x.stride(0), ptr(tokens), rows, V, stream())
+             ctx.top, ptr(x), dt(x), x.stride(0), ptr(tokens), rows, V, stream_of(x))
         return dx, None, None
 
 
@@ -200,18 +207,18 @@ def token_logprobs(logits, tokens, top=0):
         raise ValueError(f"int64 tokens {list(logits.shape[:-1])}, got {tokens.dtype} {tuple(tokens.shape)}")
     if not 0 <= top <= min(32, V):
         raise ValueError(f"{top} alternatives of {V} (at most 32)")
-    if tokens.device != logits.device:
+    if tokens.get_device() != logits.get_device():
         raise ValueError(f"logits on {logits.device}, tokens on {tokens.device}")
-    on_current(logits.device)
-    shape = tuple(tokens.shape)
+    stream_of(logits)  # refuses the CPU and another device than the current one
     if tokens.numel() == 0:  # no rows: empty results, on the graph of logits
         z = logits.sum(-1).float()
         t = logits[..., :top].float()
         return TokenLogprobs(z, z.clone(), torch.empty(t.shape, device=t.device, dtype=torch.int64) if top else None,
                              t if top else None)
-    x = logits.reshape(-1, V)
+    x = logits if logits.dim() == 2 else logits.reshape(-1, V)
     if x.stride(1) != 1:
         x = x.contiguous()
-    lp, ent, ids, top_lp = _TokenLogprobs.apply(x, tokens.reshape(-1).contiguous(), top)
-    return TokenLogprobs(lp.view(shape), ent.view(shape), ids.view(shape + (top,)) if top else None,
-                         top_lp.view(shape + (top,)) if top else None)
+    tokens = tokens.contiguous()
+    if x.requires_grad and torch.is_grad_enabled():
+        return TokenLogprobs(*_TokenLogprobs.apply(x, tokens, top))
+    return TokenLogprobs(*_token_logprobs(x, tokens, top, None))
