@@ -157,7 +157,7 @@ def call(name, *args):
 
 
 def _call(name, args):
-    rc = getattr(lib(), name)(*args)
+    rc = getattr(_lib or lib(), name)(*args)
     if rc != 0:
         raise RuntimeError(f"{name} failed ({rc}): {lib().msq_last_error().decode()}")
     return rc

@@ -138,7 +138,7 @@ def kv8_read(kc, ks, vc, vs, pos, *, first=0, rows=None, dtype=torch.bfloat16, n
     if first < 0 or rows < 0 or first + rows > S_ring or dtype not in (torch.float32, torch.bfloat16):
         raise ValueError(f"rows {first} .. {first + rows} of a ring of {S_ring} in {dtype}")
     s = stream_of(kc)
-    k = torch.empty((B, H, rows, hs), device=kc.device, dtype=dtype)
+    k = ks.new_empty((B, H, rows, hs), dtype=dtype)
     v = torch.empty_like(k)
     if rows and B and H:
         call("msq_kv8_read", dt(k), k.data_ptr(), v.data_ptr(), *cache, B, H, hs, S_ring, *rest, first, rows, s)
@@ -170,12 +170,12 @@ def relattn_decode_kv8(q, kc, ks, vc, vs, R, pos, scale, *, out=None, n_meta=N_M
         raise ValueError(f"a row's heads have to lie {hs} apart, got strides {sq} and {so}")
     s = stream_of(kc)
     if out is None:
-        out = torch.empty((B, H, hs), device=q.device, dtype=q.dtype)
+        out = q.new_empty((B, H, hs))
     if B == 0 or H == 0:
         return out
     n = L.lib().msq_relattn_decode_kv8_workspace(B, H, hs, S_ring)
     # a scratch of its own for every call: captured graphs and streams never share one
-    ws = torch.empty(n, device=q.device, dtype=torch.uint8) if n else None
+    ws = ks.new_empty(n // 4) if n else None
     call("msq_relattn_decode_kv8", dt(q), out.data_ptr(), so[0] if B > 1 else H * hs, q.data_ptr(),
          sq[0] if B > 1 else H * hs, *cache, R.data_ptr(), S_max, B, H, hs, S_ring, *rest, float(scale),
          ws.data_ptr() if n else None, n, s)

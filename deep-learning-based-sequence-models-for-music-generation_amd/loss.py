@@ -150,11 +150,11 @@ class TokenLogprobs(NamedTuple):
 
 def _token_logprobs(x, tokens, top, stats):
     """the launch on rows x [rows, V]; results in the tokens' shape"""
-    lp = torch.empty(tokens.shape, device=x.device, dtype=torch.float32)
+    lp = torch.empty_like(tokens, dtype=torch.float32)
     ent = torch.empty_like(lp)
     ids = top_lp = None
     if top:
-        ids = torch.empty(tokens.shape + (top,), device=x.device, dtype=torch.int64)
+        ids = tokens.new_empty(tokens.shape + (top,))
         top_lp = torch.empty_like(ids, dtype=torch.float32)
     rows, V = x.shape
     call("msq_token_logprobs", lp.data_ptr(), ent.data_ptr(), stats.data_ptr() if stats is not None else None,
