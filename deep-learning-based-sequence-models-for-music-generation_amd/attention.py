@@ -1,5 +1,7 @@
 """Relative-position attention launchers (HeadRelPos x n_heads,
 models/transformer/model_transformer.py:41-90) over the libmidiseq C ABI."""
+import functools
+
 import torch
 
 from . import _lib as L
@@ -145,6 +147,12 @@ def kv8_read(kc, ks, vc, vs, pos, *, first=0, rows=None, dtype=torch.bfloat16, n
     return k, v
 
 
+@functools.lru_cache(maxsize=None)
+def _kv8_scratch(B, H, hs, S_ring):
+    """floats of the attention's workspace"""
+    return L.lib().msq_relattn_decode_kv8_workspace(B, H, hs, S_ring) // 4
+
+
 def relattn_decode_kv8(q, kc, ks, vc, vs, R, pos, scale, *, out=None, n_meta=N_META, block=KV8_BLOCK):
     """One decode position of the relative attention over the 8-bit cache, whose
     newest position is pos (msq_relattn_decode_kv8): q [B, H, hs] (heads hs
@@ -173,10 +181,10 @@ def relattn_decode_kv8(q, kc, ks, vc, vs, R, pos, scale, *, out=None, n_meta=N_M
         out = q.new_empty((B, H, hs))
     if B == 0 or H == 0:
         return out
-    n = L.lib().msq_relattn_decode_kv8_workspace(B, H, hs, S_ring)
+    n = _kv8_scratch(B, H, hs, S_ring)
     # a scratch of its own for every call: captured graphs and streams never share one
-    ws = ks.new_empty(n // 4) if n else None
+    ws = ks.new_empty(n) if n else None
     call("msq_relattn_decode_kv8", dt(q), out.data_ptr(), so[0] if B > 1 else H * hs, q.data_ptr(),
          sq[0] if B > 1 else H * hs, *cache, R.data_ptr(), S_max, B, H, hs, S_ring, *rest, float(scale),
-         ws.data_ptr() if n else None, n, s)
+         ws.data_ptr() if n else None, 4 * n, s)
     return out

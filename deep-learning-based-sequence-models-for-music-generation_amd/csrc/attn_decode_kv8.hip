@@ -16,7 +16,7 @@
 
 namespace {
 
-constexpr int NT = 256, HS = KV8_MAX_HS;
+constexpr int HS = KV8_MAX_HS;
 constexpr float LOG2E = 1.44269504088896340736f;
 
 struct Args {
@@ -28,7 +28,7 @@ struct Args {
     float *po, *pml;
     const int64_t* pos;
     int64_t pos_stride, ldq, ldo, S_max;
-    int B, H, hs, S_ring, n_meta, block_log2, nblk, chunk, nsplit, remap;
+    int B, H, hs, S_ring, n_meta, block_log2, nblk, chunk, nsplit, waves, remap;
     float scale;
 };
 
@@ -79,14 +79,15 @@ template <int N> struct Row<float, N> {
 };
 template <int N> struct Codes {
     uint32_t v[N / 4];
+    // read once: not to push the rows of R out of the L2
     __device__ __forceinline__ void load(const uint8_t* p) {
         if constexpr (N == 16) {
-            const u32x4 x = *(const u32x4*)p;
+            const u32x4 x = __builtin_nontemporal_load((const u32x4*)p);
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[i] = x[i];
         } else {
-            const uint2 x = *(const uint2*)p;
-            v[0] = x.x, v[1] = x.y;
+            const uint64_t x = __builtin_nontemporal_load((const uint64_t*)p);
+            v[0] = (uint32_t)x, v[1] = (uint32_t)(x >> 32);
         }
     }
     // e4m3 is exact in bf16: two products per instruction
@@ -121,29 +122,37 @@ template <int N> struct Codes {
     }
 };
 
-template <typename T, int VPL, int LPK>
-__global__ __launch_bounds__(NT) void decode_kv8_kernel(Args a) {
+template <typename T, int VPL, int LPK, int NW>
+__global__ __launch_bounds__(64 * NW) void decode_kv8_kernel(Args a) {
     constexpr int GW = 64 / LPK;                       // keys per load of a wave
     constexpr int UN = VPL * sizeof(T) > 32 ? 2 : 4;   // loads of a wave in flight: 64 registers
-    constexpr int STEP = 4 * GW * UN;
-    __shared__ float part[4][HS];
-    __shared__ float wm[4], wl[4];
+    constexpr int STEP = NW * GW * UN;
+    __shared__ float part[NW][HS];
+    __shared__ float wm[NW], wl[NW];
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, grp = lane / LPK;
-    // the rows of the batch that read the same rows of R run side by side on one
-    // XCD ((h, chunk) pairs dealt round the 8 of them)
+    // workgroups go round the 8 XCDs: the chunks and rows of a head, which read the
+    // same rows of R, on one XCD (remap 2: 8 | H), else those of a (h, chunk) pair
+    // (remap 1); the rows of the batch side by side
     int h, c;
     int64_t b;
     if (a.remap) {
-        const int i = blockIdx.x >> 3, pair = i / a.B * 8 + (blockIdx.x & 7);
-        if (pair >= a.H * a.nsplit) return;
-        b = i % a.B;
-        h = pair / a.nsplit;
-        c = pair % a.nsplit;
+        const int x = blockIdx.x & 7, i = blockIdx.x >> 3, k = i / a.B;
+        b = i - k * a.B;
+        if (a.remap == 2) {
+            h = k / a.nsplit;
+            c = k - h * a.nsplit;
+            h = h * 8 + x;
+        } else {
+            const int pair = k * 8 + x;
+            if (pair >= a.H * a.nsplit) return;
+            h = pair / a.nsplit;
+            c = pair - h * a.nsplit;
+        }
     } else {
-        b = blockIdx.x % a.B;
         const int pair = blockIdx.x / a.B;
+        b = blockIdx.x - pair * a.B;
         h = pair / a.nsplit;
-        c = pair % a.nsplit;
+        c = pair - h * a.nsplit;
     }
     const int hs = a.hs, ctx = a.S_ring - a.n_meta;
     const int64_t bh = b * a.H + h, last = a.pos[b * a.pos_stride];
@@ -226,10 +235,12 @@ __global__ __launch_bounds__(NT) void decode_kv8_kernel(Args a) {
     }
     if (lane == 0) wm[w] = M, wl[w] = l;
     __syncthreads();
-    M = fmaxf(fmaxf(wm[0], wm[1]), fmaxf(wm[2], wm[3]));
+    M = wm[0];
+#pragma unroll
+    for (int i = 1; i < NW; ++i) M = fmaxf(M, wm[i]);
     float acc = 0.f, L = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < NW; ++i) {
         const float g = pexp(wm[i], M);
         L = fmaf(g, wl[i], L);
         if (tid < hs) acc = fmaf(g, part[i][tid], acc);
@@ -246,41 +257,84 @@ __global__ __launch_bounds__(NT) void decode_kv8_kernel(Args a) {
 // out[b, h] = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c over the chunks that hold keys
 template <typename T>
 __global__ __launch_bounds__(HS) void decode_kv8_join_kernel(Args a) {
-    const int tid = threadIdx.x, h = blockIdx.x, hs = a.hs;
-    const int64_t b = blockIdx.y, base = (b * a.H + h) * a.nsplit;
+    __shared__ float f[HS];
+    const int tid = threadIdx.x, hs = a.hs;
+    const int64_t b = blockIdx.y, bh = b * a.H + blockIdx.x, base = bh * a.nsplit;
     const f32x2* ml = (const f32x2*)a.pml + base;
-    float M = -INFINITY;
-    for (int c = 0; c < a.nsplit; ++c) M = fmaxf(M, ml[c][0]);  // an empty chunk's is -inf
-    float L = 0.f, acc = 0.f;
-    bool any = false;
-    for (int c = 0; c < a.nsplit; ++c) {
-        const f32x2 x = ml[c];
-        const float o = tid < hs ? a.po[(base + c) * hs + tid] : 0.f;  // not written where the chunk is empty
-        if (x[1] != -1.f) {
-            const float f = pexp(x[0], M);
-            L = fmaf(f, x[1], L);
-            acc = fmaf(f, o, acc);
-            any = true;
+    const float* po = a.po + base * hs + tid;
+    float M = -INFINITY, L = 0.f, acc = 0.f;
+    int any = 0;
+    for (int c0 = 0; c0 < a.nsplit; c0 += HS) {  // HS chunks at a time, one a thread
+        const int n = min(HS, a.nsplit - c0);
+        f32x2 x = {-INFINITY, -1.f};
+        if (tid < n) x = ml[c0 + tid];
+        const bool held = x[1] != -1.f;  // else the chunk is empty and its part was not written
+        f[tid] = held ? x[0] : -INFINITY;
+        any |= __syncthreads_or(held);
+        float Mn = M;
+        for (int i = 0; i < n; ++i) Mn = fmaxf(Mn, f[i]);
+        __syncthreads();
+        f[tid] = held ? pexp(x[0], Mn) : -1.f;  // (NaN stays NaN)
+        __shared__ float l[HS];
+        l[tid] = held ? x[1] : 0.f;
+        __syncthreads();
+        const float r = pexp(M, Mn);
+        M = Mn;
+        acc *= r;
+        L *= r;
+        for (int i = 0; i < n; i += 4) {
+            float o[4], g[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                g[k] = i + k < n ? f[i + k] : -1.f;
+                o[k] = tid < hs && g[k] != -1.f ? po[(int64_t)(c0 + i + k) * hs] : 0.f;
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (g[k] != -1.f) acc = fmaf(g[k], o[k], acc), L = fmaf(g[k], l[i + k], L);
         }
+        __syncthreads();
     }
-    if (tid < hs) ((T*)a.out)[b * a.ldo + (int64_t)h * hs + tid] = (T)(any ? acc / L : 0.f);
+    if (tid < hs) ((T*)a.out)[b * a.ldo + (int64_t)blockIdx.x * hs + tid] = (T)(any ? acc / L : 0.f);
 }
 
-// Chunks of a row's ring: enough workgroups for 256 CUs of four or more each, but
-// no chunk under 128 slots; whole multiples of 64 slots
-int64_t chunk_of(int64_t B, int64_t H, int64_t S_ring) {
-    const int64_t want = std::max<int64_t>(1, 4096 / (B * H));
-    const int64_t n = std::min(want, (S_ring + 127) / 128), c = (S_ring + n - 1) / n;
-    return (c + 63) / 64 * 64;
-}
-int64_t splits(int64_t B, int64_t H, int64_t S_ring) {
-    const int64_t c = chunk_of(B, H, S_ring);
-    return (S_ring + c - 1) / c;
+struct Plan {
+    int64_t chunk, nsplit;
+    int waves;
+};
+// How a row's ring is cut. A workgroup streams at its CU's share of the memory's
+// rate (some 19 KB/us of 4.8 TB/s), so a cut into n chunks takes ceil(B H n /
+// 256) / n times a whole row, and a join of some 4 us more: the n that fill one
+// to four rounds of the 256 CUs are weighed. 64 rows x 8 heads x 2054 keys of 128
+// run uncut in 53 us (in 8 chunks 57, in 32 69); 8 rows in 4 chunks 15 us (uncut
+// 24); 4 rows x 16 heads x 16385 keys of 64 in 4 chunks 36 us (uncut 89). Rows at
+// positions of their own are cut into 10 workgroups a CU, for the long ones not to
+// be left over (24 rows x 16 heads of up to 16385 keys: 125 us; uncut 186). Eight
+// waves a workgroup where each has a pass or more over the loop, else four.
+Plan plan_of(int64_t B, int64_t H, int64_t hs, int64_t S_ring, bool ragged) {
+    const int64_t U = B * H, most = std::max<int64_t>(1, S_ring / 128);
+    const double row = (double)S_ring * hs * 2 / 19e3;
+    int64_t best = 1;
+    double cost = row * ((U + 255) / 256);
+    for (int k = 1; k <= 4; ++k) {
+        const int64_t n = std::min(most, 256 * k / U);
+        if (n <= best) continue;
+        const double c = row * ((U * n + 255) / 256) / n + 4.0;
+        if (c < cost) cost = c, best = n;
+    }
+    if (ragged) best = std::max(best, std::min(most, (2560 + U - 1) / U));
+    Plan p;
+    p.chunk = ((S_ring + best - 1) / best + 31) / 32 * 32;
+    p.nsplit = (S_ring + p.chunk - 1) / p.chunk;
+    const int64_t unit = hs > 64 ? 32 : hs > 32 ? 64 : hs > 16 ? 128 : 256;  // keys of a wave in flight
+    p.waves = p.chunk >= 12 * unit && !ragged ? 8 : 4;
+    return p;
 }
 
 template <typename T, int VPL, int LPK>
 void launch_one(const Args& a, unsigned grid, hipStream_t s) {
-    hipLaunchKernelGGL((decode_kv8_kernel<T, VPL, LPK>), dim3(grid), dim3(NT), 0, s, a);
+    if (a.waves == 8) hipLaunchKernelGGL((decode_kv8_kernel<T, VPL, LPK, 8>), dim3(grid), dim3(512), 0, s, a);
+    else hipLaunchKernelGGL((decode_kv8_kernel<T, VPL, LPK, 4>), dim3(grid), dim3(256), 0, s, a);
 }
 template <typename T>
 void launch(const Args& a, unsigned grid, hipStream_t s) {
@@ -305,7 +359,7 @@ void launch(const Args& a, unsigned grid, hipStream_t s) {
 
 extern "C" size_t msq_relattn_decode_kv8_workspace(int64_t B, int64_t H, int64_t hs, int64_t S_ring) {
     if (B <= 0 || H <= 0 || hs <= 0 || S_ring <= 0) return 0;
-    const int64_t n = splits(B, H, S_ring);
+    const int64_t n = plan_of(B, H, hs, S_ring, true).nsplit;  // no fewer than with one position for all
     return n > 1 ? (size_t)(B * H * n * (hs + 2)) * sizeof(float) : 0;
 }
 
@@ -336,15 +390,17 @@ extern "C" int msq_relattn_decode_kv8(int dtype, void* out, int64_t ldo, const v
     a.B = (int)B; a.H = (int)H; a.hs = (int)hs; a.S_ring = (int)S_ring; a.n_meta = (int)n_meta;
     a.block_log2 = __builtin_ctz((unsigned)block);
     a.nblk = (int)((S_ring + block - 1) / block);
-    a.chunk = (int)chunk_of(B, H, S_ring);
-    a.nsplit = (int)splits(B, H, S_ring);
+    const Plan p = plan_of(B, H, hs, S_ring, pos_stride != 0);
+    a.chunk = (int)p.chunk;
+    a.nsplit = (int)p.nsplit;
+    a.waves = p.waves;
     MSQ_CHECK_ARG((int64_t)a.chunk * hs < (1ll << 31), "%s: a ring of %lld for %lld x %lld heads", fn, (long long)S_ring,
                   (long long)B, (long long)H);  // 32-bit offsets inside a chunk
     a.po = (float*)ws;
     a.pml = (float*)ws + B * H * a.nsplit * hs;
     a.scale = scale;
     const int64_t pairs = H * a.nsplit;
-    a.remap = pairs >= 32;  // fewer would leave XCDs without work
+    a.remap = H % 8 == 0 ? 2 : pairs >= 32;  // fewer would leave XCDs without work
     const int64_t grid = (a.remap ? (pairs + 7) / 8 * 8 : pairs) * B;
     MSQ_CHECK_ARG(grid < (1ll << 31), "%s: %lld workgroups", fn, (long long)grid);
     if (dtype == MSQ_BF16) launch<bf16>(a, (unsigned)grid, (hipStream_t)stream);

@@ -16,9 +16,14 @@ __host__ __device__ __forceinline__ int kv8_window(int64_t last, int n_meta, int
     const int64_t n = last + 1 < ctx ? last + 1 : ctx;
     return n + n_meta > 0 ? (int)(n + n_meta) : 0;
 }
+// a % n for a >= 0: by a 32-bit division wherever that does (the 64-bit one is a
+// long scalar sequence at the head of every workgroup)
+__host__ __device__ __forceinline__ int kv8_mod(int64_t a, int n) {
+    return a >> 32 ? (int)(a % n) : (int)((uint32_t)a % (uint32_t)n);
+}
 // ring offset of the window's first token (0 until the ring wraps)
 __host__ __device__ __forceinline__ int kv8_first(int64_t last, int ctx) {
-    return last + 1 > ctx ? (int)((last + 1) % ctx) : 0;
+    return last + 1 > ctx ? kv8_mod(last + 1, ctx) : 0;
 }
 __host__ __device__ __forceinline__ bool kv8_block_ok(int64_t block) {
     return block == 16 || block == 32 || block == 64 || block == 128;

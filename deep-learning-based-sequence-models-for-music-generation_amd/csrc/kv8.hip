@@ -75,12 +75,12 @@ __global__ __launch_bounds__(NT) void kv8_write_kernel(WriteArgs a) {
     // the i-th touched block: from the first new row's slot, round the ring
     int blk = i;
     if (!a.all) {
-        const int s = p0 < 0 ? (int)p0 + a.n_meta : a.n_meta + (int)(p0 % ctx);
+        const int s = p0 < 0 ? (int)p0 + a.n_meta : a.n_meta + kv8_mod(p0, ctx);
         blk = s / a.block + i;
         if (blk >= a.nblk) blk += a.n_meta / a.block - a.nblk;
     }
     const int s0 = blk * a.block, cpr = a.hs >> 3, rows = min(a.block, a.S_ring - s0), n = rows * cpr;
-    const int lm = last >= 0 ? (int)(last % ctx) : 0;
+    const int lm = last >= 0 ? kv8_mod(last, ctx) : 0;
     uint8_t* code = a.code[kv] + ((b * a.H + h) * a.S_ring + s0) * a.hs;
     float* scale = a.scale[kv] + (b * a.H + h) * a.nblk + blk;
     const T* src = (const T*)a.src[kv] + b * a.sb + (int64_t)h * a.hs;
