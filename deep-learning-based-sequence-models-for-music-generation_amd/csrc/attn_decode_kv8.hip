@@ -312,7 +312,8 @@ struct Plan {
 // be left over (24 rows x 16 heads of up to 16385 keys: 125 us; uncut 186). Eight
 // waves a workgroup where each has a pass or more over the loop, else four.
 Plan plan_of(int64_t B, int64_t H, int64_t hs, int64_t S_ring, bool ragged) {
-    const int64_t U = B * H, most = std::max<int64_t>(1, S_ring / 128);
+    // no chunk under 32 KB, what four waves have in flight at once
+    const int64_t U = B * H, most = std::max<int64_t>(1, S_ring * hs * 2 / 32768);
     const double row = (double)S_ring * hs * 2 / 19e3;
     int64_t best = 1;
     double cost = row * ((U + 255) / 256);

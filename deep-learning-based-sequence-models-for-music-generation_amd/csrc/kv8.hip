@@ -17,7 +17,7 @@
 // contents in registers between the maximum and the store, 8 values per lane
 // and chunk.
 //
-// Read. Elementwise: 8 codes per lane and pass, in window order (oldest first).
+// Read. Elementwise: 8 (fp32: 4) codes per lane and pass, in window order (oldest first).
 // Both are bound by their bytes; what is read or written once goes past the caches
 // (a prompt of 32 x 2054 rows x 8 heads of 128: 85 us without, 81 us with that).
 #include "kv8.h"
@@ -178,33 +178,44 @@ struct ReadArgs {
     int64_t pos_stride;
     int H, hs, S_ring, n_meta, block_log2, nblk, first, n;
 };
-constexpr int READ_PASSES = 2;  // rows of a workgroup, in units of the NT / (hs / 8) that its lanes take at
-                                // once (a window of 32 x 2054 rows x 8 heads of 128: 78, 65, 70, 110 us for 1, 2, 4, 8)
+constexpr int READ_PASSES = 2;  // rows of a workgroup, in units of those that its lanes take at once
+                                // (a window of 32 x 2054 rows x 8 heads of 128: 78, 65, 70, 110 us for 1, 2, 4, 8)
 
-__device__ __forceinline__ void put8(bf16* p, f32x4 a, f32x4 b) {
-    union { bf16x8 v; u32x4 u; } r;
-    r.v = (bf16x8){(bf16)a[0], (bf16)a[1], (bf16)a[2], (bf16)a[3], (bf16)b[0], (bf16)b[1], (bf16)b[2], (bf16)b[3]};
-    __builtin_nontemporal_store(r.u, (u32x4*)p);
-}
-__device__ __forceinline__ void put8(float* p, f32x4 a, f32x4 b) {
-    __builtin_nontemporal_store(a, (f32x4*)p);
-    __builtin_nontemporal_store(b, (f32x4*)(p + 4));
-}
+// 16 bytes of values per lane and store, so that a wave's store covers whole lines
+template <typename T> struct Out;
+template <> struct Out<bf16> {
+    static constexpr int N = 8;
+    typedef uint64_t code;
+    static __device__ __forceinline__ void put(bf16* p, code x, float f) {
+        const f32x4 a = kv8_dec4((uint32_t)x) * f, b = kv8_dec4((uint32_t)(x >> 32)) * f;
+        union { bf16x8 v; u32x4 u; } r;
+        r.v = (bf16x8){(bf16)a[0], (bf16)a[1], (bf16)a[2], (bf16)a[3], (bf16)b[0], (bf16)b[1], (bf16)b[2], (bf16)b[3]};
+        __builtin_nontemporal_store(r.u, (u32x4*)p);
+    }
+};
+template <> struct Out<float> {
+    static constexpr int N = 4;
+    typedef uint32_t code;
+    static __device__ __forceinline__ void put(float* p, code x, float f) {
+        __builtin_nontemporal_store(kv8_dec4(x) * f, (f32x4*)p);
+    }
+};
 
 // grid: (groups of rows, K | V x head, row of the batch)
 template <typename T>
 __global__ __launch_bounds__(NT) void kv8_read_kernel(ReadArgs a) {
+    typedef typename Out<T>::code code_t;
     const int h = blockIdx.y >> 1, kv = blockIdx.y & 1;
     const int64_t b = blockIdx.z, bh = b * a.H + h;
-    const int cpr = a.hs >> 3, ctx = a.S_ring - a.n_meta, rpp = NT / cpr;  // rows per pass
-    const int row = threadIdx.x / cpr, c = (threadIdx.x - row * cpr) * 8;
+    const int cpr = a.hs / Out<T>::N, ctx = a.S_ring - a.n_meta, rpp = NT / cpr;  // lanes of a row, rows per pass
+    const int row = threadIdx.x / cpr, c = (threadIdx.x - row * cpr) * Out<T>::N;
     if (row >= rpp) return;
     const int64_t last = a.pos[b * a.pos_stride];
     const int S = kv8_window(last, a.n_meta, ctx), shift = kv8_first(last, ctx);
     const uint8_t* code = a.code[kv] + bh * a.S_ring * a.hs + c;
     const float* scale = a.scale[kv] + bh * a.nblk;
     T* out = (T*)a.out[kv] + bh * a.n * a.hs + c;
-    uint64_t x[READ_PASSES];
+    code_t x[READ_PASSES];
     float f[READ_PASSES];
 #pragma unroll
     for (int p = 0; p < READ_PASSES; ++p) {
@@ -217,14 +228,14 @@ __global__ __launch_bounds__(NT) void kv8_read_kernel(ReadArgs a) {
                 s += shift;
                 s -= s >= a.S_ring ? ctx : 0;
             }
-            x[p] = __builtin_nontemporal_load((const uint64_t*)(code + (int64_t)s * a.hs));
+            x[p] = __builtin_nontemporal_load((const code_t*)(code + (int64_t)s * a.hs));
             f[p] = scale[s >> a.block_log2];
         }
     }
 #pragma unroll
     for (int p = 0; p < READ_PASSES; ++p) {
         const int64_t r = (int64_t)blockIdx.x * (READ_PASSES * rpp) + p * rpp + row;
-        if (r < a.n) put8(out + r * a.hs, kv8_dec4((uint32_t)x[p]) * f[p], kv8_dec4((uint32_t)(x[p] >> 32)) * f[p]);
+        if (r < a.n) Out<T>::put(out + r * a.hs, x[p], f[p]);
     }
 }
 
@@ -310,7 +321,7 @@ extern "C" int msq_kv8_read(int dtype, void* k, void* v, const void* kc, const f
     a.block_log2 = __builtin_ctz((unsigned)block);
     a.nblk = (int)msq_kv8_blocks(S_ring, block);
     a.first = (int)first; a.n = (int)rows;
-    const int64_t group = READ_PASSES * (NT / (hs / 8));
+    const int64_t group = READ_PASSES * (NT / (hs / (dtype == MSQ_BF16 ? Out<bf16>::N : Out<float>::N)));
     const dim3 grid((unsigned)((rows + group - 1) / group), (unsigned)(2 * H), (unsigned)B);
     if (dtype == MSQ_BF16) hipLaunchKernelGGL(kv8_read_kernel<bf16>, grid, dim3(NT), 0, (hipStream_t)stream, a);
     else hipLaunchKernelGGL(kv8_read_kernel<float>, grid, dim3(NT), 0, (hipStream_t)stream, a);

@@ -27,7 +27,7 @@
 
 namespace {
 
-constexpr int MAXTOP = 32, VCAP = 128, CAP = 128;
+constexpr int MAXTOP = 32, VCAP = 128, CAP = 256;  // a row of under 32 vectors fits whole
 constexpr float LOG2E = 1.44269504088896340736f;
 
 template <typename T> struct Vec { static constexpr int N = 16 / sizeof(T); };
@@ -82,17 +82,27 @@ struct Row {
         : x((const T*)base + row * ld), V(V_), off((int)(((uintptr_t)x & 15) / sizeof(T))) {}
     __device__ __forceinline__ int64_t vecs() const { return (V + off + N - 1) / N; }
     __device__ __forceinline__ int64_t at(int64_t j) const { return j * N - off; }
-    // elements outside the row read as -inf; keep: the row is read again soon
-    template <bool keep = true>
-    __device__ __forceinline__ u32x4 load(int64_t j) const {
+    __device__ __forceinline__ bool whole(int64_t j) const { return at(j) >= 0 && at(j) + N <= V; }
+    // elements outside the row read as -inf; KEEP: the row is read again soon
+    template <bool KEEP = true>
+    __device__ __forceinline__ u32x4 inner(int64_t j) const {  // of a whole vector
+        const T* p = x + at(j);
+        return KEEP ? *(const u32x4*)p : __builtin_nontemporal_load((const u32x4*)p);
+    }
+    __device__ __forceinline__ u32x4 edge(int64_t j) const {
         const int64_t i0 = at(j);
-        if (i0 >= 0 && i0 + N <= V)
-            return keep ? *(const u32x4*)(x + i0) : __builtin_nontemporal_load((const u32x4*)(x + i0));
         union { u32x4 v; T t[N]; } r;
 #pragma unroll
         for (int e = 0; e < N; ++e) r.t[e] = i0 + e >= 0 && i0 + e < V ? x[i0 + e] : (T)-INFINITY;
         return r.v;
     }
+    static __device__ __forceinline__ u32x4 none() {
+        union { u32x4 v; T t[N]; } r;
+#pragma unroll
+        for (int e = 0; e < N; ++e) r.t[e] = (T)-INFINITY;
+        return r.v;
+    }
+    __device__ __forceinline__ u32x4 load(int64_t j) const { return whole(j) ? inner(j) : edge(j); }
 };
 
 // order of the values as unsigned integers, -0 = +0, NaN largest (above +inf,
@@ -177,7 +187,7 @@ __device__ void top_slow(const Row<T>& R, int top, uint64_t* kred, uint64_t* out
 // backward pass will read the rows again (4096 fp32 rows, both passes: 162 us, 191
 // with loads past the caches; alone they cost 4096 bf16 rows 35 us, and 33 past)
 template <typename T, int NT, int NV, bool KEEP>
-__global__ __launch_bounds__(NT * rows_per_block(NT)) void token_logprobs_kernel(FwdArgs a) {
+__global__ __launch_bounds__(NT * rows_per_block(NT), NT == 1024 ? 8 : 6) void token_logprobs_kernel(FwdArgs a) {
     constexpr int W = NT / 64, N = Vec<T>::N, NR = NV ? NV : 1, UN = 4, RB = rows_per_block(NT);
     __shared__ float lmax_[RB][NT], rs_[RB][W], rt_[RB][W];
     __shared__ u32x4 vecs_[RB][VCAP];
@@ -198,15 +208,27 @@ __global__ __launch_bounds__(NT * rows_per_block(NT)) void token_logprobs_kernel
         y = a.tok[row];
         if (y >= 0 && y < a.V) xy = (float)R.x[y];
     }
-    // whether this wave's i-th vectors hold any of the row (uniform)
-    auto live = [&](int i) { return i * NT + w * 64 < nv; };
+    // whether this wave's i-th vectors hold any of the row (uniform; the count is made
+    // opaque between the passes, or the compiler copies what follows for each of its values)
+    int left = __builtin_amdgcn_readfirstlane((int)min(nv, (int64_t)1 << 30) - w * 64);
+    auto live = [&](int i) { return i * NT < left; };
     u32x4 v[NR];
     float vm[NR], m = -INFINITY;
     Sums sum;
     if constexpr (NV > 0) {
 #pragma unroll
         for (int i = 0; i < NV; ++i)
-            if (live(i)) v[i] = R.template load<KEEP>(i * NT + tid);  // past the row: -inf throughout
+            if (live(i)) v[i] = R.whole(i * NT + tid) ? R.template inner<KEEP>(i * NT + tid) : R.none();
+        // the row's first and last vector, where they are not whole
+        const int je = (int)nv - 1;
+        if (tid == 0 && !R.whole(0)) v[0] = R.edge(0);
+        if (je > 0 && tid == je % NT && !R.whole(je)) {
+            const u32x4 u = R.edge(je);
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if (i == je / NT) v[i] = u;
+        }
+        asm volatile("" : "+s"(left));
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             vm[i] = -INFINITY;
@@ -245,9 +267,11 @@ __global__ __launch_bounds__(NT * rows_per_block(NT)) void token_logprobs_kernel
         if (at < VCAP) vecs_[sub][at] = u, vec_at_[sub][at] = (uint32_t)j;
     };
     if constexpr (NV > 0) {
+        asm volatile("" : "+s"(left));
 #pragma unroll
         for (int i = 0; i < NV; ++i)
             if (live(i)) sum.template add<T>(v[i], Mf);
+        asm volatile("" : "+s"(left));
         if (a.top)
 #pragma unroll
             for (int i = 0; i < NV; ++i)
@@ -342,7 +366,7 @@ __device__ __forceinline__ u32x4 pack<bf16>(const float* d) {
 // with their own terms.
 template <typename T, int NT>
 __global__ __launch_bounds__(NT * rows_per_block(NT)) void token_logprobs_bwd_kernel(BwdArgs a) {
-    constexpr int N = Vec<T>::N, UN = 4, RB = rows_per_block(NT);
+    constexpr int N = Vec<T>::N, UN = 2, RB = rows_per_block(NT);
     const int tid = threadIdx.x % NT, w0 = tid & ~63;
     const int64_t row = a.rows - 1 - ((int64_t)blockIdx.x * RB + threadIdx.x / NT);
     if (RB > 1 && row < 0) return;
@@ -416,15 +440,13 @@ void launch_fwd(const FwdArgs& a, int64_t rows, hipStream_t s) {
     if (rows >= 1024) {
         FWD(64, 3);
         FWD(64, 9);
-        FWD(256, 5);
         FWD(256, 9);
         FWD(512, 9);
     } else {
         FWD(256, 1);
     }
     FWD(1024, 1);
-    FWD(1024, 3);
-    FWD(1024, 5);
+    FWD(1024, 2);
     FWD(1024, 9);
 #undef FWD
     hipLaunchKernelGGL((token_logprobs_kernel<T, 1024, 0, KEEP>), dim3((unsigned)rows), dim3(1024), 0, s, a);
