@@ -12,6 +12,7 @@ from oracle.fill import REAL, TINY, grammar_tokens
 from midiseq.config import Discretization, Grammar
 from midiseq.generate import generate, score
 from midiseq.loss import filtered_cross_entropy, filtered_logit, token_logprobs
+from midiseq.mamba import Mamba
 from midiseq.transformer import Transformer, TransformerConfig
 
 pytestmark = pytest.mark.gpu
@@ -136,6 +137,21 @@ def test_score_has_a_gradient():
         grads.append(g)
     # fp32 on both sides, sums of some hundred terms: well within 1e-4 of the largest
     assert ((grads[0] - grads[1]).abs().max() <= 1e-4 * grads[1].abs().max()).item()
+
+
+def test_score_of_a_mamba_model():
+    vocab, mv = TINY, 10
+    m = Mamba(d_model=128, n_layers=2, vocab_size=vocab.size, metadata_vocab_size=mv, precision="fp32").to("cuda").eval()
+    d = vocab.disc
+    gr = Grammar(Discretization(**{k: d[k] for k in ("pitch", "channel", "dyn", "length", "time", "tempo")}))
+    w, meta = tokens(2, 40, 6, vocab), torch.zeros(2, 6, dtype=torch.int64)
+    r = score(m, w, meta, grammar=gr)
+    with torch.no_grad():
+        logits = m(w[:, :-1].contiguous().cuda(), meta.cuda())
+        loss = filtered_cross_entropy(w[:, :-1].contiguous().cuda(), logits, w[:, 1:].contiguous().cuda(), gr)
+    assert r.top_ids is None and abs(loss.item() + r.logprob.mean().item()) < 1e-5 * max(1.0, loss.item())
+    with pytest.raises(ValueError, match="Transformer"):
+        generate(m, 24, w, meta, num_tokens=1, mode="cached", kv="fp8")
 
 
 def test_refusals():

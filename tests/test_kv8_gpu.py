@@ -149,6 +149,34 @@ def test_write_strides(dtype):
     assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(before, p.c))
 
 
+def test_write_padded_prompts():
+    """A batch of prompts padded to one length: the padding's rows lie behind each row's newest
+    position once the first token is written at the prompt's own end (positions taken back), and a
+    scale that they had raised falls again."""
+    g, p = rng(12), Pair(4, 2, 32, 64, 6, 16)
+    k, v = rows(g, (4, 46, 2, 32), torch.bfloat16), rows(g, (4, 46, 2, 32), torch.bfloat16)
+    for x in (k, v):
+        x[0][:, 30:] *= 1024
+        x[1][:, 30:] *= 1024
+    p.write(k, v, -6)
+    p.check()
+    at = [40, 33, 24, 9]  # prompts of 46, 39, 30 and 15 rows
+    for i in range(20):
+        p.garbage = [t.view(torch.uint8).cpu().numpy().copy() for t in (p.c[0], p.c[2])]
+        scales = [t.clone() for t in (p.c[1], p.c[3])]
+        p.write(rows(g, (4, 1, 2, 32), torch.bfloat16), rows(g, (4, 1, 2, 32), torch.bfloat16), at)
+        for j in range(2):
+            code = p.c[2 * j].view(torch.uint8).cpu().numpy()
+            for b in range(4):
+                r, w = p.o[b][j], sorted(p.o[b][j].window())
+                np.testing.assert_array_equal(okv.e4m3_value(code[b][:, w]), r.val[:, w])
+                rest = [s for s in range(p.S) if s not in w]
+                np.testing.assert_array_equal(code[b][:, rest], p.garbage[j][b][:, rest])
+                np.testing.assert_array_equal(p.c[2 * j + 1][b].cpu().numpy(), np.where(
+                    np.arange(5) == r.slot(at[b]) // 16, r.scale, scales[j][b].cpu().numpy()))
+        at = [q + 1 for q in at]
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("shape", SHAPES)
 def test_read(shape, dtype):
@@ -254,6 +282,29 @@ def test_attend_one_position(shape, pos, dtype):
                                0.25, out=out[:, 8:8 + H * hs].view(B, H, hs), n_meta=shape[4], block=shape[5])
     check_attend(p, q, R, [pos] * B, got, 0.25, dtype)
     assert (out[:, :8] == 5).all() and (out[:, 8 + H * hs:] == 5).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("hs", [16, 32, 64, 128])
+def test_cache_on_8_bytes(hs, dtype):
+    """A cache that is 8- but not 16-byte aligned takes half the codes a lane."""
+    shape, pos = (2, 3, hs, 200, 6, 64), [150, 333]
+    p, q, R = filled(shape, pos, dtype)
+    c = [t.clone() for t in p.c]
+    for i in (0, 2):
+        raw = torch.zeros(c[i].numel() + 8, device=dev, dtype=torch.uint8)
+        raw[8:] = c[i].view(torch.uint8).flatten()
+        c[i] = raw[8:].view(torch.float8_e4m3fn).view(c[i].shape)
+        assert c[i].data_ptr() % 16 == 8
+    check_attend(p, q, R, pos, A.relattn_decode_kv8(q[0], *c, R[0], torch.tensor(pos, device=dev), 0.1), 0.1, dtype)
+    k, v = rows(rng(3), (2, 2, 3, hs), dtype), rows(rng(4), (2, 2, 3, hs), dtype)
+    at = torch.tensor([q + 1 for q in pos], device=dev)
+    A.kv8_write(*c, k[0], v[0], at)
+    A.kv8_write(*p.c, k[0], v[0], at)
+    for a, b in zip(c, p.c):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    for a, b in zip(A.kv8_read(*c, at + 1), A.kv8_read(*p.c, at + 1)):
+        assert torch.equal(a, b)
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])

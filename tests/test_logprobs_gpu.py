@@ -68,6 +68,52 @@ def check_backward(x64, tokens, ids, g, dx, dtype):
     close(dx, want, tol)
 
 
+def reference(x, tok, gl, gh):
+    """the same answers in 64 bits by torch, for many rows: logprob, entropy, sorted log probabilities, gradient"""
+    lp = torch.log_softmax(x.double(), -1)
+    p = lp.exp()
+    ent = -torch.special.xlogy(p, p).sum(-1)
+    at = torch.arange(len(x), device=dev)
+    d = p * (-gl - gh * ent)[:, None] - gh[:, None] * torch.special.xlogy(p, p)
+    d[at, tok] += gl
+    return lp[at, tok], ent, lp, d
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,V", [(1025, 60), (1026, 700), (1027, 1501), (1025, 4099), (1030, 9001), (1025, 17914),
+                                    (1024, 20011), (1025, 40009), (1024, 80003), (1023, 3001)])
+def test_many_rows(rows, V, dtype):
+    """Each of the kernel's forms (by the row's length, and whether the rows are many), both passes.
+    Tolerances as above, of the tensors' largest."""
+    g = torch.Generator(dev).manual_seed(V)
+    x = (torch.randn(rows, V, device=dev, generator=g) * 3).to(dtype)
+    tok = torch.randint(0, V, (rows,), device=dev, generator=g)
+    gl, gh = torch.randn(rows, device=dev, generator=g), torch.randn(rows, device=dev, generator=g)
+    lp, ent, all_lp, d = reference(x, tok, gl.double(), gh.double())
+    leaf = x.clone().requires_grad_(True)
+    r = token_logprobs(leaf, tok, 6)
+    r0 = token_logprobs(x, tok, 6)  # the form without a gradient
+    for a, b in zip(r, r0):
+        assert torch.equal(a, b)
+    A = (V + 64) * 2.0 ** -24
+    big = lp.abs().max().item() + np.log(V)
+    assert ((r.logprob - lp).abs().max() <= A + 3 * 2.0 ** -24 * big).item()
+    assert ((r.entropy - ent).abs().max() <= A * (2 + np.log(V)) + 2.0 ** -22 * (1 + np.log(V))).item()
+    # stable: equal values by index
+    want = torch.sort(x.float(), dim=-1, descending=True, stable=True).indices[:, :6]
+    assert torch.equal(r.top_ids, want)
+    assert ((r.top_logprobs - all_lp.gather(1, want)).abs().max() <= A + 3 * 2.0 ** -24 * big).item()
+    (dx,) = torch.autograd.grad((r.logprob, r.entropy), leaf, (gl, gh))
+    g1, g2 = gl.abs()[:, None], gh.abs()[:, None]
+    alp = all_lp.abs()
+    tol = all_lp.exp() * ((A + 2.0 ** -22 * (1 + alp)) * (g1 + g2 * (1 + alp + np.log(V))) * 2)
+    tol += 2.0 ** -22 * d.abs() + 2.0 ** -126 * (1 + g1 + g2 * (1 + alp + np.log(V)))
+    if dtype == torch.bfloat16:
+        tol += 2.0 ** -8 * d.abs() * (1 + 2.0 ** -7)
+    off = (dx.double() - d).abs() - tol
+    assert (off.max() <= 0).item(), off.max().item()
+
+
 SIZES = [(1, 1), (3, 2), (5, 7), (4, 33), (2, 255), (6, 1025), (3, 4099), (2, 17914), (2, 70001), (300, 40)]
 
 
@@ -132,7 +178,7 @@ def test_broadcast_rows():
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("V", [9, 700, 5003])
+@pytest.mark.parametrize("V", [9, 700, 5003, 80003])
 def test_masks(V, dtype):
     """-inf, the type's lowest value, empty rows, one live logit, +inf and NaN, and ties of all of them."""
     g = np.random.default_rng(V)
@@ -207,6 +253,14 @@ def test_no_rows_and_one_token():
     assert dx.shape == x.shape
     r = token_logprobs(torch.randn(9, device=dev), torch.tensor(4, device=dev), 2)  # a row alone
     assert r.logprob.shape == () and r.top_ids.shape == (2,)
+
+
+def test_second_derivatives_are_refused():
+    x = torch.randn(3, 8, device=dev, requires_grad=True)
+    (g,) = torch.autograd.grad(token_logprobs(x, torch.zeros(3, dtype=torch.int64, device=dev)).logprob.sum(), x,
+                               create_graph=True)
+    with pytest.raises(RuntimeError):
+        g.sum().backward()
 
 
 def test_changed_logits_are_refused():
