@@ -114,7 +114,8 @@ def kv8_write(kc, ks, vc, vs, k, v, pos, *, n_meta=N_META, block=KV8_BLOCK):
     projection) at positions pos .. pos + T - 1 of the ring, in place
     (msq_kv8_write). pos: int64 [B], or [1] for all rows; -n_meta for a prompt
     whose first n_meta rows are metadata; below that a row is left alone.
-    Positions are written in order."""
+    Positions are written in order; a row may be taken back to an earlier one
+    (a prompt's padding, rejected tokens) while the ring has not come round."""
     shape, strides = k.shape, k.stride()
     if len(shape) != 4 or v.shape != shape or v.dtype != k.dtype or v.stride() != strides:
         raise ValueError(f"k and v are [B, T, H, hs] alike, got {k.dtype} {tuple(k.shape)} {k.stride()} and "

@@ -11,7 +11,8 @@
 // 16 codes where the head size allows it), so a wave's load covers 64 / LPK
 // consecutive slots; every such key group keeps its own running maximum, sum and
 // output (one pass, no exchange inside the loop but the LPK-lane sum of a
-// score). Groups and waves are joined at the end, chunks by a second kernel.
+// score). Groups and waves are joined at the end, the chunks of a row by a second
+// kernel.
 #include "kv8.h"
 
 namespace {
@@ -158,6 +159,7 @@ __global__ __launch_bounds__(64 * NW) void decode_kv8_kernel(Args a) {
     const int64_t bh = b * a.H + h, last = a.pos[b * a.pos_stride];
     const int S = kv8_window(last, a.n_meta, ctx), first = kv8_first(last, ctx), s0 = c * a.chunk;
     const int n = min(S - s0, a.chunk);  // keys of this chunk
+    if (n <= 0 && a.nsplit > 1) return;  // no key in this chunk (uniform)
     const int d0 = VPL * (lane % LPK);
     const bool dok = d0 < hs;
     const uint8_t* kc = a.kc + (bh * a.S_ring + s0) * hs + d0;
@@ -245,57 +247,57 @@ __global__ __launch_bounds__(64 * NW) void decode_kv8_kernel(Args a) {
         L = fmaf(g, wl[i], L);
         if (tid < hs) acc = fmaf(g, part[i][tid], acc);
     }
+    T* out = (T*)a.out + b * a.ldo + (int64_t)h * hs;
     if (a.nsplit == 1) {
         if (tid < hs) ((T*)a.out)[b * a.ldo + (int64_t)h * hs + tid] = (T)(S > 0 ? acc / L : 0.f);
         return;
     }
     const int64_t pi = bh * a.nsplit + c;
-    if (n > 0 && tid < hs) a.po[pi * hs + tid] = acc;
-    if (tid == 0) a.pml[2 * pi] = M, a.pml[2 * pi + 1] = n > 0 ? L : -1.f;  // -1: no key in this chunk
+    if (tid < hs) a.po[pi * hs + tid] = acc;
+    if (tid == 0) a.pml[2 * pi] = M, a.pml[2 * pi + 1] = L;
 }
 
-// out[b, h] = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c over the chunks that hold keys
+// out[b, h] = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c over the chunks that hold keys,
+// HS chunks at a time. (Joined instead by the workgroup that is done last: with the
+// parts written past the L2 the same time, with fences around them four to ten times
+// the whole kernel's.)
 template <typename T>
 __global__ __launch_bounds__(HS) void decode_kv8_join_kernel(Args a) {
-    __shared__ float f[HS];
+    __shared__ float f[HS], l[HS];
     const int tid = threadIdx.x, hs = a.hs;
     const int64_t b = blockIdx.y, bh = b * a.H + blockIdx.x, base = bh * a.nsplit;
     const f32x2* ml = (const f32x2*)a.pml + base;
     const float* po = a.po + base * hs + tid;
+    const int S = kv8_window(a.pos[b * a.pos_stride], a.n_meta, a.S_ring - a.n_meta);
+    const int nc = (S + a.chunk - 1) / a.chunk;
     float M = -INFINITY, L = 0.f, acc = 0.f;
-    int any = 0;
-    for (int c0 = 0; c0 < a.nsplit; c0 += HS) {  // HS chunks at a time, one a thread
-        const int n = min(HS, a.nsplit - c0);
-        f32x2 x = {-INFINITY, -1.f};
+    for (int c0 = 0; c0 < nc; c0 += HS) {
+        const int n = min(HS, nc - c0);
+        f32x2 x = {-INFINITY, 0.f};
         if (tid < n) x = ml[c0 + tid];
-        const bool held = x[1] != -1.f;  // else the chunk is empty and its part was not written
-        f[tid] = held ? x[0] : -INFINITY;
-        any |= __syncthreads_or(held);
+        f[tid] = x[0];
+        __syncthreads();
         float Mn = M;
         for (int i = 0; i < n; ++i) Mn = fmaxf(Mn, f[i]);
         __syncthreads();
-        f[tid] = held ? pexp(x[0], Mn) : -1.f;  // (NaN stays NaN)
-        __shared__ float l[HS];
-        l[tid] = held ? x[1] : 0.f;
+        f[tid] = pexp(x[0], Mn);
+        l[tid] = x[1];
         __syncthreads();
         const float r = pexp(M, Mn);
         M = Mn;
         acc *= r;
         L *= r;
         for (int i = 0; i < n; i += 4) {
-            float o[4], g[4];
+            float o[4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                g[k] = i + k < n ? f[i + k] : -1.f;
-                o[k] = tid < hs && g[k] != -1.f ? po[(int64_t)(c0 + i + k) * hs] : 0.f;
-            }
+            for (int k = 0; k < 4; ++k) o[k] = tid < hs && i + k < n ? po[(int64_t)(c0 + i + k) * hs] : 0.f;
 #pragma unroll
             for (int k = 0; k < 4; ++k)
-                if (g[k] != -1.f) acc = fmaf(g[k], o[k], acc), L = fmaf(g[k], l[i + k], L);
+                if (i + k < n) acc = fmaf(f[i + k], o[k], acc), L = fmaf(f[i + k], l[i + k], L);
         }
         __syncthreads();
     }
-    if (tid < hs) ((T*)a.out)[b * a.ldo + (int64_t)blockIdx.x * hs + tid] = (T)(any ? acc / L : 0.f);
+    if (tid < hs) ((T*)a.out)[b * a.ldo + (int64_t)blockIdx.x * hs + tid] = (T)(nc > 0 ? acc / L : 0.f);
 }
 
 struct Plan {

@@ -503,7 +503,9 @@ int msq_relattn_decode_pos(int dtype, void* out, int64_t ldo, const void* qkv, i
 int64_t msq_kv8_blocks(int64_t S_ring, int64_t block);
 /* T new rows of keys and values (dtype MSQ_F32 / MSQ_BF16; row t of batch row b
  * at k + b * ld_b + t * ld_t, head h at + h * hs) become positions pos .. pos +
- * T - 1; positions are written in order. A touched block's scale becomes the
+ * T - 1. Positions are written in order; a row may be taken back (written again
+ * from an earlier position: what then lies behind its newest one is no part of
+ * it) as long as the ring has not come round since. A touched block's scale becomes the
  * smallest 2^e, e >= -126, with |x| <= 448 * 2^e over its finite contents, new
  * rows and rows that stay; rows that stay are coded again where the scale
  * moved (exact but for codes that fall under 2^-6 of the new scale).
