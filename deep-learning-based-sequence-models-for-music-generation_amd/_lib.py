@@ -185,11 +185,11 @@ def stream_of(t):
     return torch._C._cuda_getCurrentRawStream(dev)  # current_stream(dev).cuda_stream without the object
 
 
+_DT = {torch.float32: F32, torch.bfloat16: BF16, torch.int32: MASK1}  # int32: a GEMM aux bitmask (MSQ_MASK1)
+
+
 def dt(t):
-    if t.dtype == torch.float32:
-        return F32
-    if t.dtype == torch.bfloat16:
-        return BF16
-    if t.dtype == torch.int32:  # a GEMM aux bitmask (MSQ_MASK1)
-        return MASK1
-    raise TypeError(f"unsupported dtype {t.dtype}")
+    d = _DT.get(t.dtype)
+    if d is None:
+        raise TypeError(f"unsupported dtype {t.dtype}")
+    return d

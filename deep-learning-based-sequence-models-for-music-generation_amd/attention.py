@@ -56,6 +56,7 @@ def relattn_bwd(dout, out, lse, qkv, R, B, S, H, hs, scale, dqkv=None, dR=None, 
 # ---- the decode cache in 8 bits (msq_kv8_*, msq_relattn_decode_kv8)
 
 KV8_BLOCK = 64  # slots that share a scale
+_F8, _F32, _BF16, _I64 = torch.float8_e4m3fn, torch.float32, torch.bfloat16, torch.int64
 
 
 def kv8_cache(B, H, S_ring, hs, device="cuda", block=KV8_BLOCK, layers=()):
@@ -76,23 +77,23 @@ def kv8_cache(B, H, S_ring, hs, device="cuda", block=KV8_BLOCK, layers=()):
 def _kv8_args(kc, ks, vc, vs, pos, n_meta, block):
     """the checked cache: (pointers, (B, H, hs, S_ring, n_meta, block, pos, pos_stride))"""
     shape = kc.shape
-    if kc.dtype != torch.float8_e4m3fn or vc.dtype != torch.float8_e4m3fn or len(shape) != 4 or vc.shape != shape:
+    if kc.dtype is not _F8 or vc.dtype is not _F8 or len(shape) != 4 or vc.shape != shape:
         raise ValueError(f"the cache is two float8_e4m3fn [B, H, S_ring, hs] tensors, got {kc.dtype} "
                          f"{tuple(kc.shape)} and {vc.dtype} {tuple(vc.shape)}")
     B, H, S_ring, hs = shape
     if not 0 <= n_meta < S_ring or block not in (16, 32, 64, 128):
         raise ValueError(f"a ring of {S_ring} slots, {n_meta} of them metadata, in blocks of {block}")
     want = (B, H, -(-S_ring // block))
-    if ks.dtype != torch.float32 or vs.dtype != torch.float32 or ks.shape != want or vs.shape != want:
+    if ks.dtype is not _F32 or vs.dtype is not _F32 or ks.shape != want or vs.shape != want:
         raise ValueError(f"the scales are two float32 {list(want)} tensors, got {ks.dtype} {tuple(ks.shape)} and "
                          f"{vs.dtype} {tuple(vs.shape)}")
     if not (kc.is_contiguous() and vc.is_contiguous() and ks.is_contiguous() and vs.is_contiguous()):
         raise ValueError("the cache and its scales have to be contiguous")
     n = pos.numel()
-    if pos.dtype != torch.int64 or pos.dim() > 1 or (n != 1 and n != B) or not pos.is_contiguous():
+    if pos.dtype is not _I64 or pos.dim() > 1 or (n != 1 and n != B) or not pos.is_contiguous():
         raise ValueError(f"pos is an int64 tensor of 1 or {B} positions, got {pos.dtype} {tuple(pos.shape)}")
     dev = kc.get_device()
-    if vc.get_device() != dev or ks.get_device() != dev or vs.get_device() != dev or pos.get_device() != dev:
+    if not dev == vc.get_device() == ks.get_device() == vs.get_device() == pos.get_device():
         raise ValueError("the cache, its scales and pos have to be on one device")
     return ((kc.data_ptr(), ks.data_ptr(), vc.data_ptr(), vs.data_ptr()),
             (B, H, hs, S_ring, n_meta, block, pos.data_ptr(), 0 if n == 1 else 1))
@@ -123,7 +124,7 @@ def kv8_write(kc, ks, vc, vs, k, v, pos, *, n_meta=N_META, block=KV8_BLOCK):
     cache, (B, H, hs, *rest) = _kv8_args(kc, ks, vc, vs, pos, n_meta, block)
     _kv8_beside(kc, k, v)
     T = shape[1]
-    if shape != (B, T, H, hs) or k.dtype not in (torch.float32, torch.bfloat16):
+    if shape != (B, T, H, hs) or not (k.dtype is _F32 or k.dtype is _BF16):
         raise ValueError(f"{k.dtype} {tuple(shape)} rows for a cache of {B} x {H} heads of {hs}")
     if strides[3] != 1 or (H > 1 and strides[2] != hs):
         raise ValueError(f"a token's heads have to lie {hs} apart, got strides {strides}")
@@ -159,7 +160,7 @@ def relattn_decode_kv8(q, kc, ks, vc, vs, R, pos, scale, *, out=None, n_meta=N_M
     newest position is pos (msq_relattn_decode_kv8): q [B, H, hs] (heads hs
     apart), R [H, S_max, hs] contiguous, both fp32 or bf16. Returns out [B, H,
     hs] in that type; rows that are not in use (pos < -n_meta) get zeros."""
-    if len(q.shape) != 3 or q.dtype not in (torch.float32, torch.bfloat16) or R.dtype != q.dtype:
+    if len(q.shape) != 3 or not (q.dtype is _BF16 or q.dtype is _F32) or R.dtype is not q.dtype:
         raise ValueError(f"q [B, H, hs] and R in fp32 or bf16, got {q.dtype} {tuple(q.shape)} and {R.dtype}")
     cache, (B, H, hs, S_ring, *rest) = _kv8_args(kc, ks, vc, vs, pos, n_meta, block)
     _kv8_beside(kc, q, R)
