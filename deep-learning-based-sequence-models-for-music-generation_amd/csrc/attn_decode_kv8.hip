@@ -308,10 +308,10 @@ struct Plan {
 // rate (some 19 KB/us of 4.8 TB/s), so a cut into n chunks takes ceil(B H n /
 // 256) / n times a whole row, and a join of some 4 us more: the n that fill one
 // to four rounds of the 256 CUs are weighed. 64 rows x 8 heads x 2054 keys of 128
-// run uncut in 53 us (in 8 chunks 57, in 32 69); 8 rows in 4 chunks 15 us (uncut
-// 24); 4 rows x 16 heads x 16385 keys of 64 in 4 chunks 36 us (uncut 89). Rows at
+// run uncut in 52 us (in 4 chunks 55, in 8 57); 8 rows in 4 chunks 15 us (uncut
+// 25); 4 rows x 16 heads x 16385 keys of 64 in 4 chunks 35 us (uncut 89). Rows at
 // positions of their own are cut into 10 workgroups a CU, for the long ones not to
-// be left over (24 rows x 16 heads of up to 16385 keys: 125 us; uncut 186). Eight
+// be left over (24 rows x 16 heads of up to 16385 keys: 119 us; uncut 178). Eight
 // waves a workgroup where each has a pass or more over the loop, else four.
 Plan plan_of(int64_t B, int64_t H, int64_t hs, int64_t S_ring, bool ragged) {
     // no chunk under 32 KB, what four waves have in flight at once

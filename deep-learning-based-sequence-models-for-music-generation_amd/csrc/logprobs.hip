@@ -184,8 +184,8 @@ __device__ void top_slow(const Row<T>& R, int top, uint64_t* kred, uint64_t* out
 }
 
 // NV > 0: the row in registers, NV vectors a lane; NV = 0: streamed. KEEP: a
-// backward pass will read the rows again (4096 fp32 rows, both passes: 162 us, 191
-// with loads past the caches; alone they cost 4096 bf16 rows 35 us, and 33 past)
+// backward pass will read the rows again (4096 fp32 rows, both passes: 152 us, 173
+// with loads past the caches; alone they cost 4096 bf16 rows 34 us, and 31 past)
 template <typename T, int NT, int NV, bool KEEP>
 __global__ __launch_bounds__(NT * rows_per_block(NT), NT == 1024 ? 8 : 6) void token_logprobs_kernel(FwdArgs a) {
     constexpr int W = NT / 64, N = Vec<T>::N, NR = NV ? NV : 1, UN = 4, RB = rows_per_block(NT);
@@ -361,7 +361,7 @@ __device__ __forceinline__ u32x4 pack<bf16>(const float* d) {
 // Streamed: read and written once, bound by that. Rows are taken last first, so
 // that what the forward pass read last is found in the memory-side cache, and the
 // gradient is stored past the caches, so that it stays there (4096 x 17914 fp32,
-// both passes: 196 us; last row first 189; stores past the caches 182; both 162).
+// both passes: 184 us; last row first 183; stores past the caches 160; both 152).
 // The given token's and the alternatives' elements are written again at the end,
 // with their own terms.
 template <typename T, int NT>
@@ -435,7 +435,8 @@ void launch_fwd(const FwdArgs& a, int64_t rows, hipStream_t s) {
             return;                                                                                      \
         }                                                                                                \
     } while (0)
-    // many rows: as few lanes a row as hold it, for many rows a CU; few: as many lanes as help
+    // many rows: as few lanes a row as hold it, for many rows a CU (4096 bf16 rows of 17914 with 5 alternatives:
+    // 31 us, 57 with 1024 lanes; 65536 of 568: 32, 85 with 256); few: as many lanes as help
     FWD(64, 1);
     if (rows >= 1024) {
         FWD(64, 3);
@@ -455,9 +456,11 @@ template <typename T>
 void launch_bwd(const BwdArgs& a, int64_t rows, hipStream_t s) {
     const int64_t vecs = a.V / Vec<T>::N;
     const dim3 g((unsigned)rows);
+    // long rows by 1024 lanes (rows of 17914 fp32, both passes: 4096 in 146 us, 16384 in 578; by 256 lanes 154 and
+    // 618), others by 256 (65536 rows of 17914 bf16: 1251 us, 1284 by 1024): even near 2500 vectors
     if (vecs <= 256)
         hipLaunchKernelGGL((token_logprobs_bwd_kernel<T, 64>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
-    else if (rows >= 1024) hipLaunchKernelGGL((token_logprobs_bwd_kernel<T, 256>), g, dim3(256), 0, s, a);
+    else if (rows >= 1024 && vecs <= 2560) hipLaunchKernelGGL((token_logprobs_bwd_kernel<T, 256>), g, dim3(256), 0, s, a);
     else hipLaunchKernelGGL((token_logprobs_bwd_kernel<T, 1024>), g, dim3(1024), 0, s, a);
 }
 
