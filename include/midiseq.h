@@ -509,7 +509,7 @@ int64_t msq_kv8_blocks(int64_t S_ring, int64_t block);
  * smallest 2^e, e >= -126, with |x| <= 448 * 2^e over its finite contents, new
  * rows and rows that stay; rows that stay are coded again where the scale
  * moved (exact but for codes that fall under 2^-6 of the new scale).
- * Infinities saturate, NaN stays NaN.                                        */
+ * Infinities saturate, and so do values that would round to 2^128; NaN stays. */
 int msq_kv8_write(int dtype, void* kc, float* ks, void* vc, float* vs, const void* k, const void* v, int64_t ld_b,
                   int64_t ld_t, int64_t B, int64_t T, int64_t H, int64_t hs, int64_t S_ring, int64_t n_meta,
                   int64_t block, const int64_t* pos, int64_t pos_stride, void* stream);

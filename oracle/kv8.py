@@ -71,7 +71,8 @@ class Ring:
                 fin = np.abs(c[np.isfinite(c)])
                 sc = scale_of(fin.max() if fin.size else 0.0)
                 y = c / sc
-                self.val[h, slots] = e4m3_round(np.where(np.isnan(y), y, np.clip(y, -448, 448)))
+                top = 448.0 if sc < 2.0 ** 120 else 240.0             # 256 * 2^120 is no fp32 number
+                self.val[h, slots] = e4m3_round(np.where(np.isnan(y), y, np.clip(y, -top, top)))
                 self.scale[h, g] = sc
         self.last = p0 + len(x) - 1
 

@@ -27,6 +27,17 @@ def test_oracle_scale():
         assert okv.scale_of(amax) == want
 
 
+def test_oracle_largest_values():
+    """Finite fp32 values stay finite and within 2^-4, also once they are coded again."""
+    r = okv.Ring(1, 16, 8, 0, 16)
+    x = np.array([3.4028234663852886e38, -1.9375 * 2.0 ** 127, 1.875 * 2.0 ** 127, 1.75 * 2.0 ** 127, 0, 0, 0, 0])
+    r.write(x[None, None], 0)
+    for p in (1, 2):
+        r.write(np.full((1, 1, 8), 0.5), p)
+        got = r.rows()[0, 0].astype(np.float32).astype(np.float64)
+        assert (np.abs(got - x) <= 2.0 ** -4 * np.abs(x)).all()
+
+
 @pytest.mark.parametrize("kw", [dict(hs=12), dict(hs=0), dict(hs=136), dict(block=48), dict(block=8)])
 def test_cache_refusals(kw):
     with pytest.raises(ValueError):

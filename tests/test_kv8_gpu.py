@@ -115,6 +115,26 @@ def test_write_values():
         p.check()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_largest_values(dtype):
+    """Finite values next to 2^128 come back finite, within 2^-4, and stay so when their block is written again
+    (256 at the scale 2^120 would be an infinity, and then saturate at whatever scale the others ask for)."""
+    p = Pair(1, 1, 8, 16, 0, 16)
+    big = torch.finfo(dtype).max
+    row = torch.tensor([big, -big, 1.9375 * 2.0 ** 127, -1.875 * 2.0 ** 127, 1.75 * 2.0 ** 127, -2.0 ** 127, 1.0, 0.0])
+    quiet = torch.tensor([1.0, -2.0, 3e-3, 0, 0, 0, 0, 0])
+    wild = torch.tensor([float("inf"), float("-inf"), float("nan"), big, 1.0, 0, 0, 0])
+    for i, r in enumerate([row, quiet, quiet, wild, quiet]):
+        t = r.to(dtype).view(1, 1, 1, 8)
+        p.write((t.to(dev), t.double().numpy()), (-t.to(dev), -t.double().numpy()), i)
+        p.check()
+        for out in (torch.float32, torch.bfloat16):
+            k, v = A.kv8_read(*p.c, torch.tensor([i], device=dev), n_meta=0, block=16, dtype=out, rows=1)
+            want = row.to(dtype).double()
+            for got in (k.cpu().double().view(8), -v.cpu().double().view(8)):
+                assert ((got - want).abs() <= 2.0 ** -4 * want.abs() + 2.0 ** 110).all(), got
+
+
 def test_scale_falls_again():
     """A scale follows the block's contents, down as well as up, and the old codes with it."""
     g, p = rng(3), Pair(1, 2, 16, 16, 0, 16)
