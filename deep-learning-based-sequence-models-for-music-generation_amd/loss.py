@@ -199,7 +199,8 @@ def token_logprobs(logits, tokens, top=0):
     probabilities of the ``top`` <= 32 largest logits (equal ones by index).
     logprob, entropy and top_logprobs are differentiable in logits. A row of
     nothing but -inf gives log probability -inf, entropy 0 and no gradient; NaN
-    or +inf makes its row NaN."""
+    or +inf makes its row NaN. Both passes can be captured into a graph; as with
+    every torch operator, only while no eager graph of the same leaves is alive."""
     V = logits.shape[-1] if logits.dim() else 0
     if logits.dtype not in (torch.float32, torch.bfloat16) or V == 0:
         raise ValueError(f"logits [..., V] in fp32 or bf16, got {logits.dtype} {tuple(logits.shape)}")

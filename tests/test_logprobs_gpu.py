@@ -302,6 +302,37 @@ def test_graph_and_stream():
         assert torch.equal(dx, dx2)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_backward_in_a_graph(dtype):
+    """Both passes captured, replayed over other logits, tokens and incoming gradients with eager work
+    between; the leaf has no eager graph while its backward pass is captured."""
+    g = torch.Generator(dev).manual_seed(2)
+    x = torch.randn(70, 4001, device=dev, generator=g).to(dtype).requires_grad_(True)
+    tok = torch.randint(-3, 4001, (70,), device=dev, generator=g)
+    gl, gh, gt = (torch.randn(70, *s, device=dev, generator=g) for s in ((), (), (3,)))
+
+    def both(x):
+        r = token_logprobs(x, tok, 3)
+        return [*(t.detach() for t in r), *torch.autograd.grad((r.logprob, r.entropy, r.top_logprobs), x, (gl, gh, gt))]
+
+    both(x.detach().clone().requires_grad_(True))  # everything loaded
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = both(x)
+    for _ in range(4):
+        with torch.no_grad():
+            x.copy_(torch.randn(x.shape, device=dev, generator=g))
+        tok.copy_(torch.randint(-3, 4001, (70,), device=dev, generator=g))
+        for t in (gl, gh, gt):
+            t.normal_(generator=g)
+        graph.replay()
+        got = [t.clone() for t in out]
+        torch.cuda.synchronize()
+        for a, b in zip(got, both(x.detach().clone().requires_grad_(True))):
+            assert torch.equal(a, b)
+
+
 def test_rows_past_32_bits():
     """130 000 rows of 17 920 elements: 2.3 G elements; the last rows and their gradient."""
     rows, V, ld = 130_000, 17914, 17920
