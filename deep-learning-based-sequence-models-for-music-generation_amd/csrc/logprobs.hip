@@ -379,12 +379,14 @@ __global__ __launch_bounds__(NT * rows_per_block(NT)) void token_logprobs_bwd_ke
     float c = gy;
     if (a.g_top)
         for (int k = 0; k < a.top; ++k) c += a.g_top[row * a.top + k];
-    c = -c - gh * a.ent[row];
     const bool empty = M == -INFINITY && ls == 0.f;
-    // p (c - g_H lp)
+    // -p sum g - g_H p (lp + H). No product exceeds the result's size (a loss scale may
+    // bring gradients near the largest number), and lp of a masked element, whose p is 0,
+    // is kept finite: p is 0 from lp = -104 on, H is at most log V
+    const float lsh = ls - a.ent[row];
     auto smooth = [&](float x) {
         const float d = x - M, p = __builtin_amdgcn_exp2f(fmaf(d, LOG2E, -ls2));
-        return empty ? 0.f : p * fmaf(-gh, fmaxf(d - ls, -1e30f), c);
+        return empty ? 0.f : -fmaf(p, c, gh * p * fmaxf(d - lsh, -256.f));
     };
     for (int64_t j1 = 0; j1 < nv; j1 += UN * NT) {
         const int64_t j0 = j1 + tid;
