@@ -8,6 +8,7 @@ import ctypes
 import os
 
 import torch  # noqa: F401  (loads the HIP runtime before libmidiseq)
+from torch.autograd import forward_ad
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 # MSQ_LIB_PATH: an alternate build of the same library (same-box A/B tools only)
@@ -172,6 +173,13 @@ def ptr(t):
 
 def stream():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+def has_tangent(*tensors):
+    """whether one of them carries a forward-mode tangent, which no kernel here passes on"""
+    if forward_ad._current_level < 0:  # outside every dual level no tensor does
+        return False
+    return any(forward_ad.unpack_dual(t).tangent is not None for t in tensors)
 
 
 def stream_of(t):

@@ -5,7 +5,7 @@ import functools
 import torch
 
 from . import _lib as L
-from ._lib import ptr, call, stream, dt, stream_of
+from ._lib import ptr, call, stream, dt, stream_of, has_tangent
 from .ops import workspace
 
 N_META = 6  # metadata prefix (generate_matrix, model_transformer.py:14)
@@ -107,6 +107,8 @@ def _kv8_beside(kc, *others):
             raise ValueError(f"the cache is on {kc.device}, an operand on {t.device}")
         if grad and t.requires_grad:
             raise ValueError("the 8-bit cache has no gradient: call it under torch.no_grad()")
+    if has_tangent(*others):
+        raise ValueError("the 8-bit cache has no gradient: forward-mode tangents would be lost")
 
 
 def kv8_write(kc, ks, vc, vs, k, v, pos, *, n_meta=N_META, block=KV8_BLOCK):

@@ -17,7 +17,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib as L
-from ._lib import ptr, call, stream, dt, stream_of
+from ._lib import ptr, call, stream, dt, stream_of, has_tangent
 from .config import Grammar
 from .ops import workspace
 
@@ -197,7 +197,8 @@ def token_logprobs(logits, tokens, top=0):
     filtered_logit's Z): the log probability of its token (int64 [...]; outside
     [0, V), e.g. -100: 0 and no gradient), the entropy, and the ids and log
     probabilities of the ``top`` <= 32 largest logits (equal ones by index).
-    logprob, entropy and top_logprobs are differentiable in logits. A row of
+    logprob, entropy and top_logprobs are differentiable in logits (backward once;
+    a forward-mode tangent is refused). A row of
     nothing but -inf gives log probability -inf, entropy 0 and no gradient; NaN
     or +inf makes its row NaN. Both passes can be captured into a graph; as with
     every torch operator, only while no eager graph of the same leaves is alive."""
@@ -210,6 +211,8 @@ def token_logprobs(logits, tokens, top=0):
         raise ValueError(f"{top} alternatives of {V} (at most 32)")
     if tokens.get_device() != logits.get_device():
         raise ValueError(f"logits on {logits.device}, tokens on {tokens.device}")
+    if has_tangent(logits):  # refused here: without requires_grad no autograd function would see it
+        raise NotImplementedError("token_logprobs has no forward-mode derivative")
     stream_of(logits)  # refuses the CPU and another device than the current one
     if tokens.numel() == 0:  # no rows: empty results, on the graph of logits
         z = logits.sum(-1).float()
