@@ -181,6 +181,8 @@ class _TokenLogprobs(torch.autograd.Function):
         x, tokens, stats, ent, ids = ctx.saved_tensors
         if g_lp is None and g_ent is None and g_top is None:
             return None, None, None
+        if has_tangent(*(t for t in (g_lp, g_ent, g_top) if t is not None)):
+            raise NotImplementedError("the gradient of token_logprobs has no forward-mode derivative")
         rows, V = x.shape
         # rows of the gradient as far apart as those of x where that only pads
         # them: both then meet the same 16-byte boundaries
@@ -198,10 +200,10 @@ def token_logprobs(logits, tokens, top=0):
     [0, V), e.g. -100: 0 and no gradient), the entropy, and the ids and log
     probabilities of the ``top`` <= 32 largest logits (equal ones by index).
     logprob, entropy and top_logprobs are differentiable in logits (backward once;
-    a forward-mode tangent is refused). A row of
-    nothing but -inf gives log probability -inf, entropy 0 and no gradient; NaN
-    or +inf makes its row NaN. Both passes can be captured into a graph; as with
-    every torch operator, only while no eager graph of the same leaves is alive."""
+    forward-mode tangents are refused). A row of nothing but -inf gives log
+    probability -inf, entropy 0 and no gradient; NaN or +inf makes its row NaN.
+    Both passes can be captured into a graph; as with every torch operator, only
+    while no eager graph of the same leaves is alive."""
     V = logits.shape[-1] if logits.dim() else 0
     if logits.dtype not in (torch.float32, torch.bfloat16) or V == 0:
         raise ValueError(f"logits [..., V] in fp32 or bf16, got {logits.dtype} {tuple(logits.shape)}")

@@ -116,3 +116,16 @@ def test_nan_still_spreads_over_its_row():
     r = token_logprobs(leaf, torch.tensor([1, 2, 3], device=dev))
     (dx,) = torch.autograd.grad((r.logprob, r.entropy), leaf, (torch.full((3,), 1e9, device=dev),) * 2)
     assert torch.isnan(dx[1]).all() and torch.isfinite(dx[[0, 2]]).all()
+
+
+def test_forward_over_reverse_is_refused():
+    import torch.autograd.forward_ad as fwad
+    x = torch.randn(3, 8, device=dev, requires_grad=True)
+    tok = torch.zeros(3, dtype=torch.int64, device=dev)
+    with fwad.dual_level():
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            token_logprobs(fwad.make_dual(x.detach(), torch.ones_like(x)), tok)
+        lp = token_logprobs(x, tok).logprob
+        g = fwad.make_dual(torch.ones(3, device=dev), torch.ones(3, device=dev))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.autograd.grad(lp, x, g)

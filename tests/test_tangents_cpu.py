@@ -2,13 +2,14 @@
 ordinary address, so an entry point that does not look for one would drop it in silence. Refused
 before any launch (no GPU), also under no_grad, where tangents still pass through torch's operations."""
 import contextlib
+from types import SimpleNamespace
 
 import pytest
 import torch
 import torch.autograd.forward_ad as fwad
 
 from midiseq import attention as A
-from midiseq.loss import token_logprobs
+from midiseq.loss import _TokenLogprobs, token_logprobs
 
 ZERO = torch.zeros(2, dtype=torch.int64)
 
@@ -61,3 +62,15 @@ def test_others_pass_the_check(call):
 def test_the_primal_is_taken():
     with fwad.dual_level(), pytest.raises(RuntimeError, match="GPU only"):
         score(fwad.unpack_dual(dual(2, 7)).primal)
+
+
+@pytest.mark.parametrize("at", [0, 1, 3])
+def test_tangents_of_incoming_gradients_are_refused(at):
+    """forward over reverse: the incoming gradients carry them"""
+    x = torch.zeros(2, 7)
+    ctx = SimpleNamespace(saved_tensors=(x, ZERO, torch.zeros(2, 2), torch.zeros(2), ZERO[:, None]), top=1)
+    with fwad.dual_level():
+        g = [None] * 4
+        g[at] = dual(2, 1) if at == 3 else dual(2)
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            _TokenLogprobs.backward(ctx, *g)
