@@ -405,7 +405,8 @@ extern "C" int msq_relattn_decode_kv8(int dtype, void* out, int64_t ldo, const v
     const int64_t pairs = H * a.nsplit;
     a.remap = H % 8 == 0 ? 2 : pairs >= 32;  // fewer would leave XCDs without work
     const int64_t grid = (a.remap ? (pairs + 7) / 8 * 8 : pairs) * B;
-    MSQ_CHECK_ARG(grid < (1ll << 31), "%s: %lld workgroups", fn, (long long)grid);
+    MSQ_CHECK_ARG(grid * 64 * a.waves < (1ll << 32), "%s: %lld workgroups (%lld rows x %lld heads x %d chunks), a launch "
+                  "takes under %lld", fn, (long long)grid, (long long)B, (long long)H, a.nsplit, (1ll << 26) / a.waves);
     if (dtype == MSQ_BF16) launch<bf16>(a, (unsigned)grid, (hipStream_t)stream);
     else launch<float>(a, (unsigned)grid, (hipStream_t)stream);
     MSQ_LAUNCH_CHECK();

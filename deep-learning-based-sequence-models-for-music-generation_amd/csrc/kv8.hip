@@ -297,7 +297,8 @@ extern "C" int msq_kv8_write(int dtype, void* kc, float* ks, void* vc, float* vs
     a.nb = a.all ? a.nblk : (int)nb;
     a.vec = ((ld_b | ld_t) & 7) == 0 && (((uintptr_t)k | (uintptr_t)v) & 15) == 0;
     const int64_t grid = (int64_t)a.nb * 2 * H * B;
-    MSQ_CHECK_ARG(grid < (1ll << 31), "msq_kv8_write: %lld workgroups", (long long)grid);
+    MSQ_CHECK_ARG(grid * NT < (1ll << 32), "msq_kv8_write: %lld workgroups (%d rows of the batch x %d heads x %d blocks), "
+                  "a launch takes under %lld", (long long)grid, (int)B, (int)H, a.nb, (1ll << 32) / NT);
     const int rpp = NT / (int)(hs / 8), nc = ((int)block + rpp - 1) / rpp;  // <= 8
     if (dtype == MSQ_BF16) launch_write<bf16>(a, (unsigned)grid, nc, (hipStream_t)stream);
     else launch_write<float>(a, (unsigned)grid, nc, (hipStream_t)stream);
@@ -326,6 +327,8 @@ extern "C" int msq_kv8_read(int dtype, void* k, void* v, const void* kc, const f
     a.nblk = (int)msq_kv8_blocks(S_ring, block);
     a.first = (int)first; a.n = (int)rows;
     const int64_t group = READ_PASSES * (NT / (hs / (dtype == MSQ_BF16 ? Out<bf16>::N : Out<float>::N)));
+    MSQ_CHECK_ARG((rows + group - 1) / group * NT < (1ll << 32), "msq_kv8_read: %lld rows, a launch takes under %lld",
+                  (long long)rows, (1ll << 32) / NT * group);
     const dim3 grid((unsigned)((rows + group - 1) / group), (unsigned)(2 * H), (unsigned)B);
     if (dtype == MSQ_BF16) hipLaunchKernelGGL(kv8_read_kernel<bf16>, grid, dim3(NT), 0, (hipStream_t)stream, a);
     else hipLaunchKernelGGL(kv8_read_kernel<float>, grid, dim3(NT), 0, (hipStream_t)stream, a);
