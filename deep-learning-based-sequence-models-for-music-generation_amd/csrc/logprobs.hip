@@ -425,14 +425,26 @@ __global__ __launch_bounds__(NT * rows_per_block(NT)) void token_logprobs_bwd_ke
     }
 }
 
+// A launch takes fewer than 2^32 lanes; a row up to 1024 of them. More rows go in several.
+constexpr int64_t LAUNCH_ROWS = (1ll << 22) - 1;
+template <typename T>
+T* shift(T* p, int64_t n) { return p ? p + n : p; }
+
+// the variant goes by the rows of the whole call
 template <typename T, bool KEEP>
-void launch_fwd(const FwdArgs& a, int64_t rows, hipStream_t s) {
+void launch_fwd(const FwdArgs& all, int64_t r0, int64_t n, hipStream_t s) {
+    const int64_t rows = all.rows;
+    FwdArgs a = all;
+    a.x = (const T*)a.x + r0 * a.ld;
+    a.tok += r0, a.lp += r0, a.ent += r0, a.stats = shift(a.stats, 2 * r0);
+    a.top_id = shift(a.top_id, r0 * a.top), a.top_lp = shift(a.top_lp, r0 * a.top);
+    a.rows = n;
     const int64_t vecs = (a.V + 2 * (Vec<T>::N - 1)) / Vec<T>::N;  // whatever the row's alignment
 #define FWD(NT, NV)                                                                                      \
     do {                                                                                                 \
         if (vecs <= NT * NV) {                                                                           \
             constexpr int RB = rows_per_block(NT);                                                       \
-            const dim3 g((unsigned)((rows + RB - 1) / RB));                                              \
+            const dim3 g((unsigned)((n + RB - 1) / RB));                                                 \
             hipLaunchKernelGGL((token_logprobs_kernel<T, NT, NV, KEEP>), g, dim3(NT * RB), 0, s, a);     \
             return;                                                                                      \
         }                                                                                                \
@@ -452,16 +464,22 @@ void launch_fwd(const FwdArgs& a, int64_t rows, hipStream_t s) {
     FWD(1024, 2);
     FWD(1024, 9);
 #undef FWD
-    hipLaunchKernelGGL((token_logprobs_kernel<T, 1024, 0, KEEP>), dim3((unsigned)rows), dim3(1024), 0, s, a);
+    hipLaunchKernelGGL((token_logprobs_kernel<T, 1024, 0, KEEP>), dim3((unsigned)n), dim3(1024), 0, s, a);
 }
 template <typename T>
-void launch_bwd(const BwdArgs& a, int64_t rows, hipStream_t s) {
-    const int64_t vecs = a.V / Vec<T>::N;
-    const dim3 g((unsigned)rows);
+void launch_bwd(const BwdArgs& all, int64_t r0, int64_t n, hipStream_t s) {
+    const int64_t rows = all.rows, vecs = all.V / Vec<T>::N;
+    BwdArgs a = all;
+    a.x = (const T*)a.x + r0 * a.ld, a.dx = (T*)a.dx + r0 * a.ldd;
+    a.tok += r0, a.stats += 2 * r0, a.ent += r0;
+    a.g_lp = shift(a.g_lp, r0), a.g_ent = shift(a.g_ent, r0);
+    a.g_top = shift(a.g_top, r0 * a.top), a.top_id = shift(a.top_id, r0 * a.top);
+    a.rows = n;
+    const dim3 g((unsigned)n);
     // long rows by 1024 lanes (rows of 17914 fp32, both passes: 4096 in 146 us, 16384 in 578; by 256 lanes 154 and
     // 618), others by 256 (65536 rows of 17914 bf16: 1251 us, 1284 by 1024): even near 2500 vectors
     if (vecs <= 256)
-        hipLaunchKernelGGL((token_logprobs_bwd_kernel<T, 64>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((token_logprobs_bwd_kernel<T, 64>), dim3((unsigned)((n + 3) / 4)), dim3(256), 0, s, a);
     else if (rows >= 1024 && vecs <= 2560) hipLaunchKernelGGL((token_logprobs_bwd_kernel<T, 256>), g, dim3(256), 0, s, a);
     else hipLaunchKernelGGL((token_logprobs_bwd_kernel<T, 1024>), g, dim3(1024), 0, s, a);
 }
@@ -481,8 +499,11 @@ extern "C" int msq_token_logprobs(float* logprob, float* entropy, float* stats, 
     MSQ_CHECK_ARG(top == 0 || (top_ids && top_logprobs), "%s: null pointer", fn);
     const FwdArgs a{logits, ld, V, tokens, logprob, entropy, stats, top_logprobs, top_ids, rows, (int)top};
     hipStream_t s = (hipStream_t)stream;
-    if (dtype == MSQ_BF16) stats ? launch_fwd<bf16, true>(a, rows, s) : launch_fwd<bf16, false>(a, rows, s);
-    else stats ? launch_fwd<float, true>(a, rows, s) : launch_fwd<float, false>(a, rows, s);
+    for (int64_t r = 0; r < rows; r += LAUNCH_ROWS) {
+        const int64_t n = std::min(LAUNCH_ROWS, rows - r);
+        if (dtype == MSQ_BF16) stats ? launch_fwd<bf16, true>(a, r, n, s) : launch_fwd<bf16, false>(a, r, n, s);
+        else stats ? launch_fwd<float, true>(a, r, n, s) : launch_fwd<float, false>(a, r, n, s);
+    }
     MSQ_LAUNCH_CHECK();
     return MSQ_OK;
 }
@@ -500,8 +521,11 @@ extern "C" int msq_token_logprobs_bwd(void* dlogits, int64_t ldd, const float* g
     MSQ_CHECK_ARG(top >= 0 && top <= MAXTOP, "%s: %lld alternatives (at most %d)", fn, (long long)top, MAXTOP);
     MSQ_CHECK_ARG(!g_top || (top_ids && top > 0), "%s: the alternatives' gradient needs their ids", fn);
     const BwdArgs a{logits, dlogits, ld, ldd, V, tokens, top_ids, g_logprob, g_entropy, g_top, stats, entropy, rows, (int)top};
-    if (dtype == MSQ_BF16) launch_bwd<bf16>(a, rows, (hipStream_t)stream);
-    else launch_bwd<float>(a, rows, (hipStream_t)stream);
+    for (int64_t r = (rows - 1) / LAUNCH_ROWS * LAUNCH_ROWS; r >= 0; r -= LAUNCH_ROWS) {  // last rows first
+        const int64_t n = std::min(LAUNCH_ROWS, rows - r);
+        if (dtype == MSQ_BF16) launch_bwd<bf16>(a, r, n, (hipStream_t)stream);
+        else launch_bwd<float>(a, r, n, (hipStream_t)stream);
+    }
     MSQ_LAUNCH_CHECK();
     return MSQ_OK;
 }
