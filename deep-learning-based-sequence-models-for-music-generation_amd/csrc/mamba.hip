@@ -1608,10 +1608,14 @@ __global__ __launch_bounds__(256, 2) void grad_kernel(MambaArgs a, const bf16* _
     char* sMG = smem + 3 * IMG;  // M [t][s]   | dG [t][s]
     float* sdt = (float*)(smem + 4 * IMG);
     float* scum = sdt + 64;
-    float* sdcum = scum + 64;
-    float* sddt = sdcum + 64;
-    float* sred = sddt + 64;  // 8 block-reduction slots
+    // d cum and d dt by row, a set for each wave: added up in one order at the end, so
+    // that what is rounded to bf16 from them is the same every time (one set for all
+    // four waves flipped one or a few such roundings a run)
+    float* sdcum4 = scum + 64;
+    float* sddt4 = sdcum4 + 256;
+    float* sred = sddt4 + 256;  // 8 block-reduction slots
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, il = lane & 15, g = lane >> 4;
+    float *sdcum = sdcum4 + 64 * w, *sddt = sddt4 + 64 * w;
     const Chunk kg = chunk_of(a, nch, hg);
     const int nv = kg.nval;
     const int rb = 32 * (w >> 1), cb = 32 * (w & 1);
@@ -1672,7 +1676,7 @@ __global__ __launch_bounds__(256, 2) void grad_kernel(MambaArgs a, const bf16* _
         *(u32x4*)(sXY + offd(row, 8 + ch)) = row < k.nval ? pdy[u] : (u32x4){0u, 0u, 0u, 0u};
     }
     dt_cum(a, k, zx, dt_bias, A, sdt, scum, tid);
-    if (tid < 64) sdcum[tid] = sddt[tid] = 0.f;
+    sdcum4[tid] = sddt4[tid] = 0.f;
     hdh = wave_sum_dpp(hdh);
     if (lane == 0) sred[w] = hdh;
     __syncthreads();
@@ -1829,19 +1833,19 @@ __global__ __launch_bounds__(256, 2) void grad_kernel(MambaArgs a, const bf16* _
         sred[4 + w] = gd;
     }
     __syncthreads();
-    if (tid == 0) sdcum[nv - 1] += exp_decay(cl) * (sred[0] + sred[1] + sred[2] + sred[3]);
-    __syncthreads();
     if (tid < 64) {
         // da_t = sum_{tau >= t} dcum_tau ; ddt = A da + sum_p dXS x ; d dt_raw = ddt sigmoid(raw)
         // (suffix sum = prefix scan over the reversed lanes, back through the
         // same LDS row: one wave, its LDS operations in issue order)
-        const float rv = 63 - tid < nv ? sdcum[63 - tid] : 0.f;
-        sdcum[63 - tid] = wave_scan_dpp(rv);
+        const int rt = 63 - tid;
+        float rv = ((sdcum4[rt] + sdcum4[64 + rt]) + sdcum4[128 + rt]) + sdcum4[192 + rt];
+        if (rt == nv - 1) rv += exp_decay(cl) * (sred[0] + sred[1] + sred[2] + sred[3]);
+        sdcum[rt] = wave_scan_dpp(rt < nv ? rv : 0.f);  // (wave 0's set)
         const float v = sdcum[tid];
         float gA = 0.f, gdb = 0.f;
         if (tid < nv) {
             const int64_t t = k.t0 + tid;
-            const float ddt = A * v + sddt[tid];
+            const float ddt = A * v + (((sddt4[tid] + sddt4[64 + tid]) + sddt4[128 + tid]) + sddt4[192 + tid]);
             gA = sdt[tid] * v;
             const float raw = (float)zx[(k.b * a.L + t) * a.ldz + a.d_inner + a.conv_dim + k.h] + dt_bias[k.h];
             const float draw = ddt * sigm(raw);
@@ -1884,7 +1888,7 @@ __global__ __launch_bounds__(256) void dbc_reduce_kernel(const float* __restrict
     *(f32x4*)(dxc + row * ldxc + d_inner + c) = acc;
 }
 
-constexpr size_t UTERM_LDS = IMG + 512, GRAD_LDS = 4 * IMG + 2048;  // + sdt, scum, sdcum, sddt, sred
+constexpr size_t UTERM_LDS = IMG + 512, GRAD_LDS = 4 * IMG + 2624;  // + sdt, scum, sdcum4, sddt4, sred
 
 constexpr size_t STATE_LDS = IMG + 512, OUT_LDS = 3 * IMG + 512;
 }  // namespace ssd2
