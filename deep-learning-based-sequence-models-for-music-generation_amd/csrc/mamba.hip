@@ -1163,7 +1163,7 @@ __global__ __launch_bounds__(256) void state_kernel(MambaArgs a, const bf16* __r
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
         const int e = tid + 256 * u, row = e >> 3;
-        const float f = row < k.nval ? sdt[row] * expf(cl - scum[row]) : 0.f;
+        const float f = row < k.nval ? sdt[row] * exp_decay(cl - scum[row]) : 0.f;
         float v[8];
         unpack8(xr[u], v);
 #pragma unroll
@@ -1196,7 +1196,7 @@ __global__ __launch_bounds__(256) void pass_kernel(float* __restrict__ states, c
     for (int c = 0; c < nch; ++c) {
         const float sc = st[(int64_t)c * P * N];
         st[(int64_t)c * P * N] = hcur;
-        hcur = expf(cl[c]) * hcur + sc;
+        hcur = fmaf(exp_decay(cl[c]), hcur, sc);
     }
     if (fin) fin[e] = hcur;  // state after the last position (cached decode)
 }
@@ -1339,7 +1339,7 @@ __global__ __launch_bounds__(256) void uterm_kernel(MambaArgs a, const bf16* __r
         float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         if (row < k.nval) {
             unpack8(*(const u32x4*)(dY + (k.b * a.L + k.t0 + row) * ldy + k.h * P + ch * 8), v);
-            const float et = expf(scum[row]);
+            const float et = exp_decay(scum[row]);
 #pragma unroll
             for (int q = 0; q < 8; ++q) v[q] *= et;
         }
@@ -1370,7 +1370,7 @@ __global__ __launch_bounds__(256) void rpass_kernel(float* __restrict__ U, const
     for (int c = nch - 1; c >= 0; --c) {
         const float uc = u[(int64_t)c * P * N];
         u[(int64_t)c * P * N] = d;
-        d = expf(cl[c]) * d + uc;
+        d = fmaf(exp_decay(cl[c]), d, uc);
     }
 }
 
@@ -1382,7 +1382,8 @@ __global__ __launch_bounds__(256) void rpass_kernel(float* __restrict__ U, const
 // every chunk's entry state H_c (exit gradient dH_c) that `out` / `grad` read.
 // The next chunk's x / B (dY / C) and dt rows are loaded into registers while the
 // current chunk's product runs. Same arithmetic as state -> pass (uterm -> rpass):
-// H_{c+1} = e^{cum_last_c} H_c + S_c with S_c from the same MFMA sequence.
+// H_{c+1} = e^{cum_last_c} H_c + S_c with S_c from the same MFMA sequence, the same
+// exponential (exp_decay) and one fused multiply-add, so both forms give the same bits.
 __device__ __forceinline__ Chunk chunk_at(const MambaArgs& a, int64_t bh, int c) {
     Chunk k;
     k.b = bh / a.nheads;
@@ -1488,7 +1489,7 @@ __global__ __launch_bounds__(512) void scan_fwd_kernel(MambaArgs a, const bf16* 
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) H[i][0][r] = valid ? ecl * H[i][0][r] + acc[i][0][r] : H[i][0][r];
+            for (int r = 0; r < 4; ++r) H[i][0][r] = valid ? fmaf(ecl, H[i][0][r], acc[i][0][r]) : H[i][0][r];
         // the entry state of chunk c + 1 (or the final state) is stored right after
         // the update: H is next overwritten one chunk later, so the wait the store's
         // source registers need does not also wait for the next loads
@@ -1577,7 +1578,7 @@ __global__ __launch_bounds__(256) void scan_bwd_kernel(MambaArgs a, const bf16* 
 #pragma unroll
             for (int j = 0; j < 2; ++j)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) D[i][j][r] = valid ? ecl * D[i][j][r] + acc[i][j][r] : D[i][j][r];
+                for (int r = 0; r < 4; ++r) D[i][j][r] = valid ? fmaf(ecl, D[i][j][r], acc[i][j][r]) : D[i][j][r];
         // exit gradient of chunk c - 1 (chunk 0's entry gradient goes to the scratch dh0)
         store_d(c > 0 ? U + (bh * nch + c - 1) * (int64_t)(P * N) : dh0 + bh * (int64_t)(P * N));
     };

@@ -1,5 +1,6 @@
-"""The bf16 SSD passes give the same bits every time: what they hand on in bf16 is rounded from sums
-in one order, so that no rounding near a tie falls differently from run to run."""
+"""The bf16 SSD passes give the same bits every time, and their two forms (the fused scans, and the
+kernels per chunk with passes of their own) the same bits as each other: what they hand on in bf16
+is rounded from sums in one order, so that no rounding near a tie falls differently from run to run."""
 import pytest
 import torch
 
@@ -51,3 +52,13 @@ def test_runs_repeat_bitwise(B, T, H):
     for _ in range(15):
         for a, b in zip(first, passes(d)):
             assert torch.equal(a, b), int((a != b).sum())
+
+
+@pytest.mark.parametrize("B,T,H", SHAPES)
+def test_scan_forms_agree_bitwise(B, T, H, monkeypatch):
+    d = data(B, T, H, 1)
+    monkeypatch.delenv("MSQ_MAMBA_SSD_3K", raising=False)
+    fused = passes(d)
+    monkeypatch.setenv("MSQ_MAMBA_SSD_3K", "1")
+    for a, b in zip(fused, passes(d)):
+        assert torch.equal(a, b), int((a != b).sum())
