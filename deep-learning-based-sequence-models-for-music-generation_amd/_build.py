@@ -17,17 +17,10 @@ LIB = os.path.join(HERE, "libmidiseq.so")
 ARCH = os.environ.get("MSQ_OFFLOAD_ARCH", "gfx950")
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = ["-O3", "-fPIC", "-std=c++17", f"--offload-arch={ARCH}", "-I", INC, "-Wno-unused-result"]
-# no packed fp32 instructions: hipcc -O3 makes v_pk_{add,mul,fma}_f32 from ordinary
-# float code, and some of their forms have given wrong results on this hardware
-NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
-# These sources are built without that flag, as they always were: tests pin pairs of their
-# paths to each other within 1e-5, closer than one bf16 rounding that falls differently,
-# and the flag moves such roundings (with it test_mamba_fused_scan_matches_three_kernel_path
-# fails, and test_rccl_world1_bucket_path in about one run of seven; no run of either
-# failed without it). Every other source is built with it.
-PACKED_FP32 = ("attn_bwd5.hip", "attn_decode.hip", "attn_dq.hip", "attn_exact.hip", "attn_flash.hip", "attn_fwd3.hip",
-               "data.hip", "dropout.hip", "gemm.hip", "gemm256.hip", "gemm256p.hip", "gemm_skinny.hip", "loss.hip",
-               "mamba.hip", "mamba_step.hip", "midi.hip", "rowops.hip", "sample.hip")
+# no packed fp32 instructions in any source: hipcc -O3 makes v_pk_{add,mul,fma}_f32 from
+# ordinary float code, and some of their forms have given wrong results on this hardware
+# (the host pass warns that it does not know the feature)
+FLAGS += ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 
 
 def _sources():
@@ -50,8 +43,7 @@ def _stale(target, deps):
 def _compile(src):
     obj = os.path.join(OBJ, os.path.basename(src) + ".o")
     if _stale(obj, [src] + _headers()):
-        flags = FLAGS if os.path.basename(src) in PACKED_FP32 else FLAGS + NO_PACKED_FP32
-        cmd = [HIPCC] + flags + ["-c", src, "-o", obj]
+        cmd = [HIPCC] + FLAGS + ["-c", src, "-o", obj]
         if src.endswith(".cpp"):
             cmd = [HIPCC, "-O3", "-fPIC", "-std=c++17", "-I", INC, "-c", src, "-o", obj]
         r = subprocess.run(cmd, capture_output=True, text=True)
