@@ -51,7 +51,7 @@ import torch.distributed as dist
 
 from . import _lib as L
 from ._lib import ptr, call, stream, dt
-from .config import Grammar
+from .config import Grammar, N_META
 from .loss import filtered_logit, grammar_table, token_logprobs
 from .ops import workspace
 
@@ -232,11 +232,21 @@ def score(model, token_ids, meta_ids, top=0, grammar: Grammar = None, device="cu
     T of token_ids [B, T + 1] (T <= block_len) under the reference's filtered
     distribution softmax(Z), Z = filtered_logit(tokens 0 .. T-1, logits) (train.py:
     133-138), the loss.TokenLogprobs [B, T]: log probability, entropy and the
-    ``top`` alternatives. The mean of -logprob is the training loss of the rows."""
-    dev = torch.device(device)
+    ``top`` alternatives. The mean of -logprob is the training loss of the rows.
+    token_ids and meta_ids [B, N_META] are int64 ids of the model's vocabularies; rows
+    of one length, without padding (Z is normalised over the row's positions, so
+    padding would count: score rows of different lengths in calls of their own)."""
+    cfg, dev = model.engine.cfg, torch.device(device)
+    if token_ids.dim() != 2 or token_ids.shape[1] < 2:
+        raise ValueError(f"score needs rows of two tokens or more, got {tuple(token_ids.shape)}")
+    if meta_ids.shape != (token_ids.shape[0], N_META):
+        raise ValueError(f"meta_ids [{token_ids.shape[0]}, {N_META}], got {tuple(meta_ids.shape)}")
+    for name, ids, n in (("token_ids", token_ids, cfg.vocab_size), ("meta_ids", meta_ids, cfg.metadata_vocab_size)):
+        if ids.dtype != torch.int64:
+            raise ValueError(f"{name} have to be int64, not {ids.dtype}")
+        if ((ids < 0) | (ids >= n)).any():  # the embedding reads its table at them
+            raise ValueError(f"{name} outside [0, {n})")
     token_ids = token_ids.to(dev)
     src, trg = token_ids[:, :-1].contiguous(), token_ids[:, 1:].contiguous()
-    if src.shape[1] == 0:
-        raise ValueError("score needs rows of two tokens or more")
     logits = model.engine.forward(src, meta_ids.to(dev).contiguous(), save=False)
     return token_logprobs(filtered_logit(src, logits, grammar), trg, top)
