@@ -401,6 +401,8 @@ class TransformerEngine:
         B, T = idx.shape
         if T + N_META > cfg.s_max:
             raise ValueError(f"sequence of {T} tokens exceeds block_len {cfg.block_len}")
+        if cache is not None and (T > cache.ctx or B != cache.B):  # before anything is written to it
+            raise ValueError(f"prefill of {B} x {T} tokens for a cache of {cache.B} x {cache.ctx}")
         A = self.acts(B, T, save)
         A.gen += 1
         d, H, hs, S = cfg.n_embd, cfg.n_heads, cfg.head_size, T + N_META
@@ -496,8 +498,6 @@ class TransformerEngine:
             torch.cuda.current_stream(self.device).wait_event(zero_ev)
             A.bwd_zeroed = self.side_zeroed = True
         if cache is not None:
-            if T > cache.ctx:
-                raise ValueError(f"prefill of {T} tokens exceeds the cache context {cache.ctx}")
             cache.ring.fill_(float("-inf"))
             cache.part_valid = False
             cache.ring[:, :T].copy_(A.logits.view(B, T, cfg.v_pad))

@@ -165,3 +165,23 @@ def test_refusals():
         score(m, src[:, :1], meta)
     with pytest.raises(ValueError, match="head size"):
         model(dict(n_embd=24, n_heads=2, n_layer=1, block_len=24), "fp32", TINY, 10).engine.decode_cache(1, 24, kv="fp8")
+
+
+@pytest.mark.parametrize("kv", [None, "fp8"])
+def test_a_refused_prefill_leaves_the_cache(kv):
+    """A prompt that the cache cannot hold is refused before a key of it is written: the next step is
+    what it would have been."""
+    hp = dict(n_embd=64, n_heads=2, n_layer=2, block_len=40)
+    m = model(hp, "fp32", TINY, 10)
+    eng, toks, meta = m.engine, tokens(2, 40, 8, TINY).cuda(), torch.zeros(2, 6, dtype=torch.int64, device="cuda")
+    rows = []
+    with torch.no_grad():
+        for disturbed in (False, True):
+            c = eng.decode_cache(2, 20, kv)
+            eng.forward(toks[:, :20], meta, save=False, cache=c)
+            if disturbed:
+                for bad in (toks[:, 5:30], toks[:1, :20]):
+                    with pytest.raises(ValueError, match="prefill"):
+                        eng.forward(bad, meta[:len(bad)], save=False, cache=c)
+            rows.append(torch.stack([eng.step(toks[:, t].contiguous(), c).clone() for t in range(20, 24)]))
+    assert torch.equal(rows[0], rows[1])
