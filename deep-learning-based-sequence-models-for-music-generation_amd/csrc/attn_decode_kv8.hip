@@ -247,7 +247,6 @@ __global__ __launch_bounds__(64 * NW) void decode_kv8_kernel(Args a) {
         L = fmaf(g, wl[i], L);
         if (tid < hs) acc = fmaf(g, part[i][tid], acc);
     }
-    T* out = (T*)a.out + b * a.ldo + (int64_t)h * hs;
     if (a.nsplit == 1) {
         if (tid < hs) ((T*)a.out)[b * a.ldo + (int64_t)h * hs + tid] = (T)(S > 0 ? acc / L : 0.f);
         return;

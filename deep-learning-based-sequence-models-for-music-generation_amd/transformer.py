@@ -254,9 +254,9 @@ class TransformerDecodeCache:
         nst = L.lib().msq_ring_state_bytes(B, cfg.vocab_size, self.RB)
         self.ring_state = torch.empty(nst, device=device, dtype=torch.uint8)
         self.ring_blk = self.ring_state[nst - 16:nst - 8].view(torch.int64)
-        # partials of the split decode attention (msq_relattn_decode)
-        self.attn_ws = torch.empty(L.lib().msq_relattn_decode_workspace(B, H, self.S_ring), device=device,
-                                   dtype=torch.uint8)
+        # partials of the split decode attention (msq_relattn_decode; the 8-bit one takes scratch of its own)
+        self.attn_ws = None if self.kv8 else torch.empty(L.lib().msq_relattn_decode_workspace(B, H, self.S_ring),
+                                                         device=device, dtype=torch.uint8)
         self.length = 0  # tokens absorbed (sequence positions 0 .. length-1)
         # graph-replayed steps (TransformerEngine.step): the position of the
         # next step on the device (advanced by msq_ring_step), the logits row of
