@@ -118,7 +118,11 @@ def kv8_write(kc, ks, vc, vs, k, v, pos, *, n_meta=N_META, block=KV8_BLOCK):
     (msq_kv8_write). pos: int64 [B], or [1] for all rows; -n_meta for a prompt
     whose first n_meta rows are metadata; below that a row is left alone.
     Positions are written in order; a row may be taken back to an earlier one
-    (a prompt's padding, rejected tokens) while the ring has not come round."""
+    (a prompt's padding, rejected tokens) while the ring has not come round. An
+    element is off by at most 2^-4 of its value plus 2^-9 of the largest scale
+    that its block has had since it was written, taken-back rows' among them:
+    padding that is far larger than the prompt's last rows costs them (zeros cost
+    nothing)."""
     shape, strides = k.shape, k.stride()
     if len(shape) != 4 or v.shape != shape or v.dtype != k.dtype or v.stride() != strides:
         raise ValueError(f"k and v are [B, T, H, hs] alike, got {k.dtype} {tuple(k.shape)} {k.stride()} and "
@@ -160,8 +164,9 @@ def _kv8_scratch(B, H, hs, S_ring):
 def relattn_decode_kv8(q, kc, ks, vc, vs, R, pos, scale, *, out=None, n_meta=N_META, block=KV8_BLOCK):
     """One decode position of the relative attention over the 8-bit cache, whose
     newest position is pos (msq_relattn_decode_kv8): q [B, H, hs] (heads hs
-    apart), R [H, S_max, hs] contiguous, both fp32 or bf16. Returns out [B, H,
-    hs] in that type; rows that are not in use (pos < -n_meta) get zeros."""
+    apart, rows a multiple of 8 elements), R [H, S_max, hs] contiguous, both fp32
+    or bf16 and 16-byte aligned. Returns out [B, H, hs] in that type, or fills out
+    (any alignment); rows that are not in use (pos < -n_meta) get zeros."""
     if len(q.shape) != 3 or not (q.dtype is _BF16 or q.dtype is _F32) or R.dtype is not q.dtype:
         raise ValueError(f"q [B, H, hs] and R in fp32 or bf16, got {q.dtype} {tuple(q.shape)} and {R.dtype}")
     cache, (B, H, hs, S_ring, *rest) = _kv8_args(kc, ks, vc, vs, pos, n_meta, block)

@@ -6,13 +6,15 @@
 // slots is touched when one of its slots takes a new row; its contents after
 // the write are C(r) = x(r) for new rows and code(r) * scale for the rows that
 // stay, its scale is the smallest power of two 2^e (e >= -126) with
-// |C| <= 448 * 2^e over its finite contents, and code(r) = e4m3(C(r) / 2^e):
-// a function of the block's contents alone, so the order of writes does not
-// matter and a scale falls again once a large row has been overwritten. A power
-// of two costs no accuracy against amax / 448 (e4m3 keeps 3 bits of mantissa
-// down to 2^-6 of the scale, 16 octaves below its largest value) and makes the
-// re-coding of the rows that stay exact, except where a code falls below 2^-6
-// of the new scale: each element is rounded once, not once per step.
+// |C| <= 448 * 2^e over its finite contents, and code(r) = e4m3(C(r) / 2^e). The
+// scale is a function of C alone and falls again once a large row has been
+// overwritten. A power of two costs no accuracy against amax / 448 (e4m3 keeps 3
+// bits of mantissa down to 2^-6 of the scale, 15 octaves below its largest value)
+// and makes the re-coding of the rows that stay exact, except where a code falls
+// below 2^-6 of the new scale and is rounded again, to a multiple of 2^-9 of it;
+// what that takes does not come back when the scale falls. Only a scale above
+// all those the block had before can do it, and each is at least twice the last:
+// an element is off by at most 2^-4 |x| + 2^-9 of the largest scale since.
 // One workgroup per (touched block, K | V, head, row of the batch), the block's
 // contents in registers between the maximum and the store, 8 values per lane
 // and chunk.

@@ -30,8 +30,9 @@ Cached mode (``mode="cached"``):
   window's cached logits rows. oracle/transformer.py CachedTransformer
   restates these semantics; tests/test_decode_cached_gpu.py pins the build to it.
   ``kv="fp8"`` holds the ring's keys and values in 8 bits (e4m3 codes, a
-  power-of-two scale per 64 slots and head): half the bytes a step reads, at one
-  rounding of 2^-4 relative per key / value element.
+  power-of-two scale per 64 slots and head): half the bytes a step reads. An
+  element is off by at most 2^-4 of its value plus 2^-9 of the largest scale that
+  its 64 slots have had since (a scale is at most 1 / 224 of their largest value).
 
 Sharded decode (``group=``): the global batch of world x B
 prompts is split by rows over the ranks of a process group, one model

@@ -508,7 +508,9 @@ int64_t msq_kv8_blocks(int64_t S_ring, int64_t block);
  * it) as long as the ring has not come round since. A touched block's scale becomes the
  * smallest 2^e, e >= -126, with |x| <= 448 * 2^e over its finite contents, new
  * rows and rows that stay; rows that stay are coded again where the scale
- * moved (exact but for codes that fall under 2^-6 of the new scale).
+ * moved (exact but for codes that fall under 2^-6 of the new scale): an element
+ * is off by at most 2^-4 of its value plus 2^-9 of the largest scale of its
+ * block since it was written.
  * Infinities saturate, and so do values that would round to 2^128; NaN stays. */
 int msq_kv8_write(int dtype, void* kc, float* ks, void* vc, float* vs, const void* k, const void* v, int64_t ld_b,
                   int64_t ld_t, int64_t B, int64_t T, int64_t H, int64_t hs, int64_t S_ring, int64_t n_meta,
@@ -523,7 +525,8 @@ int msq_kv8_read(int dtype, void* k, void* v, const void* kc, const float* ks, c
  * and values: out[b, h] = softmax_j((q.k_j + q.R[w(j)]) * scale) . v_j over the
  * window of row b's newest position pos; q [B, ldq] and out [B, ldo] with head h
  * at h * hs, R [H, S_max, hs], all in dtype; w(j) = key j's place in the window.
- * ws of msq_relattn_decode_kv8_workspace(...) bytes, 16-B aligned (0: none).  */
+ * q and R 16-B aligned, ldq a multiple of 8. ws of
+ * msq_relattn_decode_kv8_workspace(...) bytes, 16-B aligned (0: none).        */
 size_t msq_relattn_decode_kv8_workspace(int64_t B, int64_t H, int64_t hs, int64_t S_ring);
 int msq_relattn_decode_kv8(int dtype, void* out, int64_t ldo, const void* q, int64_t ldq, const void* kc,
                            const float* ks, const void* vc, const float* vs, const void* R, int64_t S_max, int64_t B,
