@@ -129,3 +129,53 @@ def test_forward_over_reverse_is_refused():
         g = fwad.make_dual(torch.ones(3, device=dev), torch.ones(3, device=dev))
         with pytest.raises(NotImplementedError, match="forward-mode"):
             torch.autograd.grad(lp, x, g)
+
+
+def check(x, tok, dtype, seed=0):
+    """both passes within the bounds above"""
+    g = torch.Generator(dev).manual_seed(seed)
+    gl, gh = torch.randn(len(x), device=dev, generator=g), torch.randn(len(x), device=dev, generator=g)
+    leaf = x.clone().requires_grad_(True)
+    r = token_logprobs(leaf, tok)
+    (dx,) = torch.autograd.grad((r.logprob, r.entropy), leaf, (gl, gh))
+    want, ent, lp, d = exact(x, tok, gl.double(), gh.double())
+    _, tol, tol_ent = bounds(x, lp, ent, dtype)
+    tol = tol[torch.arange(len(x), device=dev), tok]
+    assert ((r.logprob.double() - want).abs() <= tol).all(), ((r.logprob.double() - want).abs() / tol).max().item()
+    off = ((r.entropy.double() - ent).abs() / tol_ent).max().item()
+    assert off <= 1, off
+    off = ((dx.double() - d).abs() / gradient_bound(x, lp, ent, d, gl.double().abs()[:, None], gh.double(), dtype)).max().item()
+    assert off <= 1, off
+    assert tol.max().item() < 2e-4  # (the bounds are as tight as meant)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows", [7, 1029])
+@pytest.mark.parametrize("V", [60, 700, 1501, 4099, 9001, 17914, 20011, 36001, 80003])
+def test_every_form_is_tight(rows, V, dtype):
+    g = torch.Generator(dev).manual_seed(V)
+    x = (torch.randn(rows, V, device=dev, generator=g) * 3).to(dtype)
+    check(x, torch.randint(0, V, (rows,), device=dev, generator=g), dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [5000, 36001, 80003, 400_009])
+def test_running_maximum(V, dtype):
+    """Rows whose maximum rises (or falls) all along, whose largest value is the last or the first of a pass, and rows
+    of a low plateau with a high end: a wrong rescale or a vector left out shows in the sum."""
+    ramp = torch.linspace(0, 12, V, device=dev)
+    x = torch.stack([ramp, ramp.flip(0), torch.where(ramp < 6, -4.0, ramp), (ramp * 2 - 12).abs(), ramp * 0 - 7.5,
+                     torch.where(torch.arange(V, device=dev) == V - 1, 8.0, 0.0),
+                     torch.where(torch.arange(V, device=dev) == 0, 8.0, 0.0)]).to(dtype)
+    check(x, torch.tensor([V - 1, 0, 5, V // 2, V // 3, V - 1, 1], device=dev), dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [1, 2, 8, 9, 63, 511, 4096, 17914, 40009, 80003])
+def test_equal_values_give_log_V(V, dtype):
+    """Every term is 1 and their sum exact, so only the logarithm is rounded: two units of it."""
+    x = torch.full((3, V), -2.75, device=dev, dtype=dtype)
+    r = token_logprobs(x, torch.tensor([0, V - 1, V // 2], device=dev))
+    tol = 2 * 2.0 ** (math.floor(math.log2(max(math.log(V), 2.0 ** -20))) - 23)
+    for got, want in ((r.logprob, -math.log(V)), (r.entropy, math.log(V))):
+        assert ((got.double() - want).abs() <= tol).all(), (got, want)
