@@ -22,7 +22,10 @@
 // for values in no order). It is found by bisection over the upper 16 bits of the
 // values' order, with a ballot a bit. The vectors that hold such elements are
 // listed in LDS, the elements ranked by (value, index). A row of many equal
-// values may list more than fit; it is then searched k times (top_slow).
+// values, or whose values above a large tie lie in fewer than k sets of lanes, may
+// list more than fit; it is then searched k times (top_slow: 4096 bf16 rows of 17914
+// with 127 events above 0 elsewhere, 32 alternatives: 1.08 ms; 39 us for values in
+// no order, and 55 in fp32, where the 127 lie in 32 vectors).
 #include "common.h"
 
 namespace {

@@ -5,7 +5,7 @@ set -e
 src=$1; out=$2; shift 2
 P=deep-learning-based-sequence-models-for-music-generation_amd
 tmp=$(mktemp -d /tmp/varXXXX)
-/opt/rocm/bin/hipcc -O3 -fPIC -std=c++17 --offload-arch=gfx950 -I include -Wno-unused-result "$@" -c "$P/$src" -o "$tmp/v.o"
+/opt/rocm/bin/hipcc -O3 -fPIC -std=c++17 --offload-arch=gfx950 -I include -Wno-unused-result -Xclang -target-feature -Xclang -packed-fp32-ops "$@" -c "$P/$src" -o "$tmp/v.o"
 objs=$(ls $P/build/*.o | grep -v "/$(basename $src).o$")
 mkdir -p "$(dirname $out)"
 /opt/rocm/bin/hipcc -shared -fPIC --offload-arch=gfx950 -o "$out" $objs "$tmp/v.o"

@@ -1,5 +1,5 @@
 // Adam update variants at the cfg-2 parameter count (154.9 M fp32 params + bf16
-// shadow): times each with HIP events. Build: hipcc --offload-arch=gfx950 -O3
+// shadow): times each with HIP events. Build: hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3
 // tools/lab/adam_lab.hip -o tools/lab/adam_lab
 #include <hip/hip_runtime.h>
 #include <hip/hip_bf16.h>

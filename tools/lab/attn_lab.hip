@@ -1,5 +1,5 @@
 // Ablation harness for the attention forward v2 (not part of the library).
-// Build: hipcc --offload-arch=gfx950 -O3 -std=c++17 -I include tools/lab/attn_lab.hip -o tools/lab/attn_lab
+// Build: hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -std=c++17 -I include tools/lab/attn_lab.hip -o tools/lab/attn_lab
 #include "../../deep-learning-based-sequence-models-for-music-generation_amd/csrc/attn_fwd3.hip"
 #include <cstdio>
 

@@ -1,5 +1,5 @@
 // Ablation harness for the 256x256 GEMM tile (not part of the library).
-// Build: hipcc --offload-arch=gfx950 -O3 -std=c++17 -I include tools/lab/gemm256_lab.hip -o tools/lab/gemm256_lab
+// Build: hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -std=c++17 -I include tools/lab/gemm256_lab.hip -o tools/lab/gemm256_lab
 // Runs the FFN1 forward shape (65728 x 4096 x 1024, bf16 out) under each LAB
 // switch combination and prints ms / TFLOP/s.
 #include "../../deep-learning-based-sequence-models-for-music-generation_amd/csrc/gemm256.hip"

@@ -1,7 +1,7 @@
 // Timing harness for the streaming filtered-CE passes at the train step's
 // size (B 32, T 2048, V 17914, bf16 logits, ld 17920); not part of the
 // library. Build:
-//   hipcc --offload-arch=gfx950 -O3 -std=c++17 -I include tools/lab/loss_lab.hip -o tools/lab/loss_lab
+//   hipcc --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -O3 -std=c++17 -I include tools/lab/loss_lab.hip -o tools/lab/loss_lab
 #include "../../deep-learning-based-sequence-models-for-music-generation_amd/csrc/loss.hip"
 #include <cstdio>
 #include <vector>
