@@ -401,8 +401,8 @@ class TransformerEngine:
         B, T = idx.shape
         if T + N_META > cfg.s_max:
             raise ValueError(f"sequence of {T} tokens exceeds block_len {cfg.block_len}")
-        if cache is not None and (T > cache.ctx or B != cache.B):  # before anything is written to it
-            raise ValueError(f"prefill of {B} x {T} tokens for a cache of {cache.B} x {cache.ctx}")
+        if cache is not None and T > cache.ctx:  # before anything is written to it
+            raise ValueError(f"prefill of {T} tokens exceeds the cache context {cache.ctx}")
         A = self.acts(B, T, save)
         A.gen += 1
         d, H, hs, S = cfg.n_embd, cfg.n_heads, cfg.head_size, T + N_META
@@ -460,7 +460,8 @@ class TransformerEngine:
             if cache is not None:
                 kv = A.qkv[k].view(B, S, 3, H, hs)
                 if cache.kv8:
-                    kv8_write(*cache.layer8(l), kv[:, :, 1], kv[:, :, 2], cache.prefill_pos)
+                    kv8 = kv.expand(cache.B, -1, -1, -1, -1)  # (one prompt for all rows, as the copies below)
+                    kv8_write(*cache.layer8(l), kv8[:, :, 1], kv8[:, :, 2], cache.prefill_pos)
             if cache is not None and not cache.kv8:
                 cache.k[l][:, :, :S].copy_(kv[:, :, 1].transpose(1, 2))
                 cache.v[l][:, :, :S].copy_(kv[:, :, 2].transpose(1, 2))

@@ -180,8 +180,24 @@ def test_a_refused_prefill_leaves_the_cache(kv):
             c = eng.decode_cache(2, 20, kv)
             eng.forward(toks[:, :20], meta, save=False, cache=c)
             if disturbed:
-                for bad in (toks[:, 5:30], toks[:1, :20]):
-                    with pytest.raises(ValueError, match="prefill"):
-                        eng.forward(bad, meta[:len(bad)], save=False, cache=c)
+                with pytest.raises(ValueError, match="prefill"):
+                    eng.forward(toks[:, 5:30], meta, save=False, cache=c)
+                with pytest.raises(RuntimeError, match="size"):  # three rows for two
+                    eng.forward(toks[[0, 1, 0], 1:21], meta[[0, 1, 0]], save=False, cache=c)
             rows.append(torch.stack([eng.step(toks[:, t].contiguous(), c).clone() for t in range(20, 24)]))
+    assert torch.equal(rows[0], rows[1])
+
+
+@pytest.mark.parametrize("kv", [None, "fp8"])
+def test_one_prompt_for_all_rows(kv):
+    """One prompt prefills every row of a cache."""
+    hp = dict(n_embd=64, n_heads=2, n_layer=2, block_len=40)
+    m = model(hp, "fp32", TINY, 10)
+    eng, toks, meta = m.engine, tokens(1, 24, 8, TINY).cuda(), torch.zeros(3, 6, dtype=torch.int64, device="cuda")
+    rows = []
+    with torch.no_grad():
+        for n in (1, 3):
+            c = eng.decode_cache(3, 30, kv)
+            eng.forward(toks[:, :20].expand(n, 20), meta[:n], save=False, cache=c)
+            rows.append(torch.stack([eng.step(toks[:, t].expand(3).contiguous(), c).clone() for t in range(20, 24)]))
     assert torch.equal(rows[0], rows[1])
