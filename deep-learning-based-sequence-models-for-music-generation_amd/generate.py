@@ -245,6 +245,8 @@ def score(model, token_ids, meta_ids, top=0, grammar: Grammar = None, device="cu
     for name, ids, n in (("token_ids", token_ids, cfg.vocab_size), ("meta_ids", meta_ids, cfg.metadata_vocab_size)):
         if ids.dtype != torch.int64:
             raise ValueError(f"{name} have to be int64, not {ids.dtype}")
+        if ids.is_cuda and torch.cuda.is_current_stream_capturing():
+            continue  # (no looking at them while a graph is captured)
         if ((ids < 0) | (ids >= n)).any():  # the embedding reads its table at them
             raise ValueError(f"{name} outside [0, {n})")
     token_ids = token_ids.to(dev)

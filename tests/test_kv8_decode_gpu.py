@@ -201,3 +201,24 @@ def test_one_prompt_for_all_rows(kv):
             eng.forward(toks[:, :20].expand(n, 20), meta[:n], save=False, cache=c)
             rows.append(torch.stack([eng.step(toks[:, t].expand(3).contiguous(), c).clone() for t in range(20, 24)]))
     assert torch.equal(rows[0], rows[1])
+
+
+def test_score_in_a_graph():
+    """Captured, the ids are not looked at; replays over other rows equal the eager calls."""
+    m = model(dict(n_embd=64, n_heads=2, n_layer=2, block_len=24), "fp32", TINY, 10)
+    d = TINY.disc
+    gr = Grammar(Discretization(**{k: d[k] for k in ("pitch", "channel", "dyn", "length", "time", "tempo")}))
+    sets = [tokens(3, 25, s, TINY).cuda() for s in range(5)]
+    rows, meta = sets[0].clone(), torch.zeros(3, 6, dtype=torch.int64, device="cuda")
+    score(m, rows, meta, 2, gr)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = score(m, rows, meta, 2, gr)
+    for s in sets:
+        rows.copy_(s)
+        graph.replay()
+        got = [t.clone() for t in out]
+        torch.cuda.synchronize()
+        for a, b in zip(got, score(m, s, meta, 2, gr)):
+            assert torch.equal(a, b)
